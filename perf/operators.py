@@ -274,7 +274,7 @@ def run(state):
         xp = s["xp"]
         pages = (s["k"], s["v"], s["table"], s["start"], s["length"])
         if c["op"] == "append":
-            xp.kv_append(s["qkv"], *pages, n_heads_q=c["heads"], rope=s.get("rope"), out=s["q"])
+            xp.kv_append(s["qkv"], *pages, n_heads_q=c["heads"], rope=s.get("rope"), out=s["q"] if c["rope"] else None)
             return (s["q_seen"], s["k_seen"], s["v_seen"]) if c["rope"] else (s["k_seen"], s["v_seen"])
         xp.paged_attention(s["q"], *pages, max_q=s["max_q"], divisor=math.sqrt(c["head_dim"]), softcap=c["cap"],
                            window=c["window"], shared=c["shared"], out=s["out"])
