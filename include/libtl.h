@@ -151,6 +151,27 @@ typedef struct tl_gemm_desc {
   float norm_eps;
 } tl_gemm_desc;
 
+/* A ragged batch over one layer of a paged KV cache, the argument block of tl_kv_append and
+ * tl_paged_attention. The cache is n_pages pages of page_size positions (a power of two, 16 to
+ * 4096); position p of sequence s lies in slot p % page_size of page page_table[s * ld_table +
+ * p / page_size]. The batch's rows are those of its sequences one after another: rows q_start[s]
+ * .. q_start[s+1] - 1 belong to sequence s, whose length with them is kv_len[s], so they sit at
+ * its last positions. q_start[0] is 0 and rows at or past q_start[n_seqs] are padding, neither
+ * read nor written. page_table, q_start and kv_len are read on the device when the kernels run (a
+ * captured step replays with the lengths of its time); entries of page_table that no position in
+ * use needs may hold anything. A bound or a page index outside its range touches no memory
+ * outside the tensors and is reported as TL_ERR_BAD_INPUT by the next synchronising call. */
+typedef struct tl_paged_desc {
+  void* k_pages; void* v_pages;   /* [n_pages, n_heads_kv, page_size, head_dim], 16-byte aligned */
+  int64_t n_pages, page_size, n_heads_q, n_heads_kv, head_dim; /* head_dim 32, 64, 128 or 256 */
+  const int32_t* page_table;      /* [n_seqs, table_cols], rows ld_table apart */
+  int64_t table_cols, ld_table;
+  const int32_t* q_start;         /* [n_seqs + 1] */
+  const int32_t* kv_len;          /* [n_seqs] */
+  int64_t n_seqs, n_rows;         /* n_rows: rows of the call's tensors, padding included */
+  int32_t dtype;                  /* TL_F32 or TL_BF16, of rows and pages */
+} tl_paged_desc;
+
 /* ---- runtime ------------------------------------------------------------------------ */
 int tl_version(void);
 /* Message of the last failed call on this thread ("" if none). */
@@ -389,6 +410,37 @@ int tl_attention_fwd_noalloc(tl_ctx* ctx, const void* q, const void* k, const vo
                              int64_t seq_q, int64_t seq_k, int64_t head_dim, int64_t ld_out,
                              int64_t offset, float divisor, int32_t causal,
                              int64_t kv_capacity, int32_t dtype);
+
+/* ---- ragged serving over a paged KV cache ----------------------------------------------- */
+/* Writes the keys and values of a QKV product's rows into the pages of their sequences, rotated by
+ * their positions on the way. qkv [n_rows, (Hq + 2 Hkv) D] holds [Q | K | V], row pitch ld_qkv;
+ * with rope_table (float [2, rope_rows, D/2]: cos then sin of positions 0 .., as tl_rope_table
+ * fills it) keys are rotated (rotate-half) and the rotated queries written to q_out [n_rows,
+ * Hq D], row pitch ld_q; without it (NULL, rope_rows 0) keys are written as they are and q_out is
+ * NULL: the queries stay in qkv. qkv and q_out must not overlap. A row whose position the table
+ * lacks is not written (TL_ERR_BAD_INPUT, as for the batch's bounds). Two sequences of a batch
+ * must not write the same page. Rows and row pitches are 16-byte aligned. No reference
+ * counterpart (its generation recomputes the window, demo.ipynb:1526-1533). */
+int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* qkv, int64_t ld_qkv,
+                 void* q_out, int64_t ld_q, const void* rope_table, int64_t rope_rows);
+/* Causal attention of a ragged batch over its pages: out[t, h D ..] = sum_j p_j v_j over the
+ * positions j <= p of row t's sequence (p the row's position), with window > 0 only those with
+ * j > p - window; p = softmax of f(q . k_j / divisor), f(s) = softcap tanh(s / softcap) when
+ * softcap > 0. q and out are [n_rows, Hq D] with row pitches ld_q and ld_out; query head h reads
+ * kv head h / (Hq / Hkv). max_q is the most rows that a sequence of the batch has (more are
+ * TL_ERR_BAD_INPUT, and the rest of that sequence is not written); it picks the kernel, so pass
+ * 1 for a batch of single tokens. A row that sees no position gives zeros. Values at positions of
+ * a sequence that its rows may not see reach no result, unless they are infinite or NaN and lie
+ * before a row of the same call that may.
+ * shared > 0 (a multiple of page_size, no window): the sequences begin with the same `shared`
+ * positions, held by the same pages (checked on the device), and every row lies behind them;
+ * a batch of few rows then reads them once for all. Results are those of shared = 0 up to
+ * rounding. q, out and their row pitches are 16-byte aligned. No reference counterpart. */
+int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const void* q, int64_t ld_q,
+                       void* out, int64_t ld_out, int64_t max_q, float divisor, float softcap,
+                       int64_t window, int64_t shared);
+/* x[i] += delta for n int32 on the device (advances the lengths of a batch inside a graph). */
+int tl_i32_add(tl_ctx* ctx, int32_t* x, int64_t n, int32_t delta);
 
 #ifdef __cplusplus
 }

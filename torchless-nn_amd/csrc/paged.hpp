@@ -1,0 +1,61 @@
+// Ragged batches over a paged KV cache: what the kernels of paged*.hip are given, and how they read
+// a sequence's bounds and pages. All of it lives in device memory, where a step that was captured
+// once finds the lengths of the step that it replays, so none of it can be checked on the host:
+// every value is held to its range here, and one outside it is latched in the status word.
+#pragma once
+
+#include "tl_internal.hpp"
+
+namespace tl {
+
+// bits of the context's status word
+enum : int32_t { kBadSequence = 4, kBadPage = 8, kBadPosition = 16, kBadShare = 32 };
+
+struct PagedBatch {
+  const int32_t* table;  // [n_seqs, cols], rows ld_table apart
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  int64_t ld_table;
+  int cols, n_seqs, n_rows, n_pages;
+  int page_shift;  // log2 of the positions in a page
+  int Hq, Hkv;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void latch(int32_t* status, int32_t bit) { atomicOr(status, bit); }
+
+// One sequence: its rows [row0, row0 + n) of the batch, and its length with them.
+struct PagedSeq {
+  int row0, n, len;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, bool report) {
+  const int a = b.q_start[s], e = b.q_start[s + 1], l = b.kv_len[s];
+  PagedSeq q;
+  q.row0 = min(max(a, 0), b.n_rows);
+  q.n = min(max(e, q.row0), b.n_rows) - q.row0;
+  q.len = min(max(l, 0), b.cols << b.page_shift);
+  if (report && (a < 0 || e < a || e > b.n_rows || l != q.len)) latch(b.status, kBadSequence);
+  return q;
+}
+
+// The page that holds position `pos` (within the table) of a sequence; page 0 for an index that the
+// cache does not have.
+__device__ __forceinline__ int paged_page(const PagedBatch& b, const int32_t* row, int pos, bool report) {
+  const int id = row[min(pos >> b.page_shift, b.cols - 1)];
+  if ((uint32_t)id < (uint32_t)b.n_pages) return id;
+  if (report) latch(b.status, kBadPage);
+  return 0;
+}
+
+// Reports, by a whole wave, a sequence that does not begin with the batch's `shared` first positions:
+// other pages than sequence 0's, or a row inside them.
+__device__ __forceinline__ void check_shared(const PagedBatch& b, int s, const PagedSeq& q, int shared, int lane) {
+  bool bad = q.n > 0 && q.len - q.n < shared;
+  for (int j = lane; j < (shared >> b.page_shift); j += 64) bad |= b.table[s * b.ld_table + j] != b.table[j];
+  if (__any(bad) && lane == 0) latch(b.status, kBadShare);
+}
+
+// Checks a descriptor and turns it into the kernels' form.
+int paged_batch(tl_ctx* ctx, const tl_paged_desc* d, PagedBatch* b);
+
+}  // namespace tl

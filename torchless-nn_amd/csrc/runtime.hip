@@ -127,7 +127,11 @@ static int check_status_word(tl_ctx* ctx) {
     TL_CHECK_HIP(hipMemcpy(ctx->status, &zero, sizeof(zero), hipMemcpyHostToDevice));
     return fail(TL_ERR_BAD_INPUT, "a kernel saw invalid input (status 0x%x): %s", word,
                 (word & 1) ? "token id out of range [0, vocab)"
-                : (word & 2) ? "gather index out of range" : "unknown");
+                : (word & 2) ? "gather index out of range"
+                : (word & 4) ? "a sequence's rows or length outside the batch's tensors"
+                : (word & 8) ? "page index outside the cache"
+                : (word & 16) ? "position past the RoPE table"
+                : (word & 32) ? "sequences do not share the pages they are said to share" : "unknown");
   }
   return TL_OK;
 }

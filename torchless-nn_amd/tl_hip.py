@@ -143,6 +143,9 @@ _GEMM_DESC = struct.Struct("@" + "".join(
     for _, t in _GemmDesc._fields_) + "0q")
 assert _GEMM_DESC.size == ctypes.sizeof(_GemmDesc)
 
+# tl_paged_desc, field for field
+_PAGED_DESC = struct.Struct("@PPqqqqqPqqPPqqi0q")
+
 _P, _I32, _I64, _F32, _F64, _SZ = (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
                                    ctypes.c_float, ctypes.c_double, ctypes.c_size_t)
 # name -> argtypes; every function returns int (tl_status) unless listed in _RESTYPES.
@@ -207,6 +210,9 @@ SIGNATURES = {
     "tl_rope2_dev": [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I32],
     "tl_i64_add": [_P, _P, _I64],
     "tl_ids_append": [_P, _P, _P, _I64, _I64, _I64, _P, _I64],
+    "tl_kv_append": [_P, _P, _P, _I64, _P, _I64, _P, _I64],
+    "tl_paged_attention": [_P, _P, _P, _I64, _P, _I64, _I64, _F32, _F32, _I64, _I64],
+    "tl_i32_add": [_P, _P, _I64, _I32],
 }
 _RESTYPES = {"tl_last_error": ctypes.c_char_p}
 
@@ -1063,6 +1069,98 @@ def ids_append(ids: DeviceTensor, hist: DeviceTensor, pos: DeviceTensor, pos_bas
     check(lib_.tl_ids_append(h, ids.ptr, hist.ptr, rows, hist.pitch, cols, _position_ptr(pos),
                              int(pos_base)))
     _wrote(hist)
+
+
+def i32_add(x: DeviceTensor, delta: int):
+    """x += delta on the device for a contiguous int32 tensor (stream-ordered)."""
+    if x.dtype is not int32 or not x.contiguous:
+        raise ValueError("i32_add takes a contiguous int32 tensor")
+    lib_, h = _c()
+    check(lib_.tl_i32_add(h, x.ptr, x.size, int(delta)))
+    _wrote(x)
+
+
+def _paged_desc(rows, k_pages, v_pages, page_table, q_start, kv_len, n_heads_q):
+    """The tl_paged_desc of a call over `rows` rows, its operands' shapes checked."""
+    if len(k_pages.shape) != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("pages are two tensors [pages, kv heads, page size, head dim]")
+    if not (k_pages.contiguous and v_pages.contiguous):
+        raise ValueError("pages must be contiguous")
+    if rows.dtype is not k_pages.dtype or rows.dtype is not v_pages.dtype:
+        raise ValueError("rows and pages must share a dtype")
+    if not (page_table.dtype is q_start.dtype is kv_len.dtype is int32):
+        raise ValueError("page_table, q_start and kv_len must be int32")
+    seqs = kv_len.size
+    if len(page_table.shape) != 2 or page_table.shape[0] != seqs or q_start.size != seqs + 1:
+        raise ValueError("expected page_table [seqs, pages], q_start [seqs + 1] and kv_len [seqs]")
+    if not (q_start.contiguous and kv_len.contiguous):
+        raise ValueError("q_start and kv_len must be contiguous")
+    n_pages, hkv, page, d = k_pages.shape
+    return _PAGED_DESC.pack(k_pages.ptr, v_pages.ptr, n_pages, page, n_heads_q, hkv, d, page_table.ptr,
+                            page_table.shape[1], page_table.pitch, q_start.ptr, kv_len.ptr, seqs, rows.nrows,
+                            rows.dtype.code)
+
+
+def kv_append(qkv: DeviceTensor, k_pages: DeviceTensor, v_pages: DeviceTensor, page_table: DeviceTensor,
+              q_start: DeviceTensor, kv_len: DeviceTensor, *, n_heads_q, rope=None, out=None) -> DeviceTensor:
+    """Keys and values of a QKV product's rows qkv [N, (Hq + 2 Hkv) D] written into the pages
+    k_pages / v_pages [P, Hkv, page, D] of their sequences: rows q_start[s] .. q_start[s+1] - 1 are
+    sequence s's last ones, its length with them kv_len[s], its pages page_table[s]. With `rope` (the
+    float table [2, R, D/2] of positions 0 ..) queries and keys are rotated; returns the queries
+    [N, Hq D]: the rotated ones (in `out` if given), or a view of qkv's columns."""
+    desc = _paged_desc(qkv, k_pages, v_pages, page_table, q_start, kv_len, n_heads_q)
+    hkv, d = k_pages.shape[1], k_pages.shape[3]
+    n, wq = qkv.nrows, n_heads_q * d
+    if len(qkv.shape) != 2 or qkv.ncols != wq + 2 * hkv * d:
+        raise ValueError(f"qkv must be [rows, {wq + 2 * hkv * d}], got {qkv.shape}")
+    if rope is None:
+        if out is not None:
+            raise ValueError("queries are written only with a RoPE table")
+        lib_, h = _c()
+        rc = lib_.tl_kv_append(h, desc, qkv.ptr, qkv.pitch, None, 0, None, 0)
+        if rc:
+            check(rc)
+        _wrote(k_pages, v_pages)
+        return DeviceTensor((n, wq), qkv.dtype, pitch=qkv.pitch, buf=qkv.buf, offset=qkv.offset)
+    if rope.dtype is not float32 or len(rope.shape) != 3 or rope.shape[0] != 2 or rope.shape[2] * 2 != d \
+            or not rope.contiguous:
+        raise ValueError("the RoPE table must be contiguous float32 [2, positions, D/2]")
+    if out is None:
+        out = DeviceTensor._alloc((n, wq), qkv.dtype, n, wq)
+    elif out.shape != (n, wq) or out.dtype is not qkv.dtype:
+        raise ValueError(f"out must be {qkv.dtype} [{n}, {wq}], got {out}")
+    lib_, h = _c()
+    rc = lib_.tl_kv_append(h, desc, qkv.ptr, qkv.pitch, out.ptr, out.pitch, rope.ptr, rope.shape[1])
+    if rc:
+        check(rc)
+    _wrote(out, k_pages, v_pages)
+    return out
+
+
+def paged_attention(q: DeviceTensor, k_pages: DeviceTensor, v_pages: DeviceTensor, page_table: DeviceTensor,
+                    q_start: DeviceTensor, kv_len: DeviceTensor, *, max_q, divisor, softcap=0.0, window=0,
+                    shared=0, out=None) -> DeviceTensor:
+    """Causal attention of a ragged batch's queries q [N, Hq D] over the pages of their sequences (the
+    batch as in kv_append, its keys and values appended) -> [N, Hq D]. `max_q`: the most rows that a
+    sequence has here; `softcap` c > 0 caps scores as c tanh(s / c); `window` w > 0 lets position p see
+    p - w + 1 .. p only; `shared`: the sequences begin with this many positions (whole pages) in the
+    same pages, read once for all by a batch of few rows a sequence."""
+    d = k_pages.shape[-1]
+    n, wq = q.nrows, q.ncols
+    if len(q.shape) != 2 or wq % d:
+        raise ValueError(f"q must be [rows, heads x {d}], got {q.shape}")
+    desc = _paged_desc(q, k_pages, v_pages, page_table, q_start, kv_len, wq // d)
+    if out is None:
+        out = DeviceTensor._alloc((n, wq), q.dtype, n, wq)
+    elif out.shape != (n, wq) or out.dtype is not q.dtype:
+        raise ValueError(f"out must be {q.dtype} [{n}, {wq}], got {out}")
+    lib_, h = _c()
+    rc = lib_.tl_paged_attention(h, desc, q.ptr, q.pitch, out.ptr, out.pitch, max_q, divisor, softcap, window,
+                                 shared)
+    if rc:
+        check(rc)
+    out.buf.version += 1
+    return out
 
 
 class Graph:
