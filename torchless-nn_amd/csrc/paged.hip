@@ -1,7 +1,4 @@
-// Ragged serving over a paged KV cache: the append of a QKV product's rows to the pages, and the
-// attention that reads them.
-#include <algorithm>
-
+// The append of a ragged batch's QKV rows to a paged KV cache.
 #include "paged.hpp"
 
 namespace tl {
@@ -41,8 +38,7 @@ int paged_batch(tl_ctx* ctx, const tl_paged_desc* d, PagedBatch* b) {
   return TL_OK;
 }
 
-// A tensor of d->n_rows rows: 16-byte aligned rows that do not overlap.
-static int check_rows(const tl_paged_desc* d, const void* p, int64_t ld, int64_t cols, const char* what) {
+int paged_rows(const tl_paged_desc* d, const void* p, int64_t ld, int64_t cols, const char* what) {
   TL_REQUIRE(p, "null pointer");
   TL_REQUIRE(ld >= cols, "row pitch of %s smaller than its %lld columns", what, (long long)cols);
   const int64_t vec = 16 / (int64_t)dtype_size(d->dtype);
@@ -55,24 +51,6 @@ static int check_rows(const tl_paged_desc* d, const void* p, int64_t ld, int64_t
 // ---------------------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------------------
-// The sequence that row t belongs to, by a whole wave: the last s with q_start[s] <= t, found by
-// 64 probes a round (one round up to 64 sequences, two up to 4096). n_seqs for a row of none.
-__device__ __forceinline__ int seq_of_row(const PagedBatch& b, int t, int lane) {
-  int lo = 0, n = b.n_seqs;  // q_start[lo] <= t as far as probed; the answer is in [lo, lo + n)
-  int hits = 0;
-  while (true) {
-    const int step = (n + 63) >> 6;
-    const int at = lo + (lane + 1) * step;
-    const bool hit = at <= lo + n && at <= b.n_seqs && b.q_start[at] <= t;
-    hits = __popcll(__ballot(hit));
-    if (step == 1) break;
-    lo += hits * step;
-    n = min(step, b.n_seqs - lo);
-    if (n <= 0) break;
-  }
-  return min(lo + (n > 0 ? hits : 0), b.n_seqs);
-}
-
 // Rows of a workgroup; each wave finds the place of one row of four.
 constexpr int kAppendRows = 4;
 
@@ -157,96 +135,9 @@ __global__ void i32_add_kernel(int32_t* x, int64_t n, int32_t delta) {
   if (i < n) x[i] += delta;
 }
 
-// ---------------------------------------------------------------------------------------
-// attention
-// ---------------------------------------------------------------------------------------
-struct PagedAttn {
-  PagedBatch b;
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
-  int64_t ld_q, ld_out;
-  int max_q, window, shared;  // window 0: none
-  float divisor, cap;
-};
-
-// One wave per (row, query head): each lane takes a key of 64, then an element of the output.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_attention_simple_kernel(PagedAttn p) {
-  __shared__ float qs[D];
-  const int lane = threadIdx.x;
-  const int t = blockIdx.x / p.b.Hq, h = blockIdx.x % p.b.Hq;
-  const int s = seq_of_row(p.b, t, lane);
-  if (s >= p.b.n_seqs) return;
-  const PagedSeq q = paged_seq(p.b, s, lane == 0);
-  const int i = t - q.row0;
-  if (i < 0 || i >= q.n) return;
-  if (p.shared > 0) check_shared(p.b, s, q, p.shared, lane);
-  if (i >= p.max_q) {
-    if (lane == 0) latch(p.b.status, kBadSequence);
-    return;
-  }
-  const int pos = q.len - q.n + i;
-  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  const int32_t* row = p.b.table + s * p.b.ld_table;
-  const T* qr = (const T*)p.q + t * p.ld_q + h * D;
-  for (int d = lane; d < D; d += 64) qs[d] = Elem<T>::load(qr + d);
-  __syncthreads();
-  const int hk = h / (p.b.Hq / p.b.Hkv), mask = (1 << p.b.page_shift) - 1;
-  constexpr int E = (D + 63) / 64;
-  float o[E] = {}, m = -INFINITY, l = 0.f;
-  for (int j0 = first; j0 <= pos; j0 += 64) {
-    const int j = j0 + lane;
-    float sc = -INFINITY;
-    int64_t at = 0;
-    if (j <= pos) {
-      const int64_t page = paged_page(p.b, row, j, true);
-      at = (((page * p.b.Hkv + hk) << p.b.page_shift) + (j & mask)) * D;
-      float a = 0.f;
-      for (int d = 0; d < D; ++d) a += qs[d] * Elem<T>::load((const T*)p.k + at + d);
-      sc = a / p.divisor;
-      if (p.cap > 0.f) sc = p.cap * tanhf(sc / p.cap);
-    }
-    const float mn = fmaxf(m, wave_max(sc));
-    const float e = expf(sc - mn), al = expf(m - mn);
-    l = l * al + wave_sum(e);
-    m = mn;
-#pragma unroll
-    for (int x = 0; x < E; ++x) o[x] *= al;
-    const int n = min(64, pos + 1 - j0);
-    for (int y = 0; y < n; ++y) {
-      const float w = __shfl(e, y, 64);
-      const int64_t a = (int64_t)__shfl((long long)at, y, 64);
-#pragma unroll
-      for (int x = 0; x < E; ++x)
-        if (x * 64 + lane < D) o[x] += w * Elem<T>::load((const T*)p.v + a + x * 64 + lane);
-    }
-  }
-  T* orow = (T*)p.out + t * p.ld_out + h * D;
-#pragma unroll
-  for (int x = 0; x < E; ++x)
-    if (x * 64 + lane < D) Elem<T>::store(orow + x * 64 + lane, l > 0.f ? o[x] / l : 0.f);
-}
-
 }  // namespace tl
 
 using namespace tl;
-
-// Calls f with a D of the descriptor's head_dim as a type.
-template <int D>
-struct HeadDim {
-  static constexpr int value = D;
-};
-template <typename F>
-static void for_head_dim(int64_t d, F f) {
-  switch (d) {
-    case 32: f(HeadDim<32>{}); break;
-    case 64: f(HeadDim<64>{}); break;
-    case 128: f(HeadDim<128>{}); break;
-    default: f(HeadDim<256>{}); break;
-  }
-}
 
 extern "C" int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* qkv, int64_t ld_qkv,
                             void* q_out, int64_t ld_q, const void* rope_table, int64_t rope_rows) {
@@ -257,13 +148,13 @@ extern "C" int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* 
   if (rc) return rc;
   const int64_t D = desc->head_dim, wq = desc->n_heads_q * D, w = wq + 2 * desc->n_heads_kv * D;
   if (desc->n_rows == 0 || desc->n_seqs == 0) return TL_OK;
-  rc = check_rows(desc, qkv, ld_qkv, w, "qkv");
+  rc = paged_rows(desc, qkv, ld_qkv, w, "qkv");
   if (rc) return rc;
   const double es = (double)dtype_size(desc->dtype);
   if (rope_table) {
     TL_REQUIRE(rope_rows > 0 && rope_rows <= (1LL << 30), "bad RoPE table length");
     TL_REQUIRE(((uintptr_t)rope_table & 15u) == 0, "the RoPE table must be 16-byte aligned");
-    rc = check_rows(desc, q_out, ld_q, wq, "q_out");
+    rc = paged_rows(desc, q_out, ld_q, wq, "q_out");
     if (rc) return rc;
     const uintptr_t x = (uintptr_t)qkv, y = (uintptr_t)q_out;
     const uintptr_t xe = x + (uintptr_t)(((desc->n_rows - 1) * ld_qkv + w) * es);
@@ -287,45 +178,6 @@ extern "C" int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* 
           (const float*)rope_table, (int)rope_rows);
   });
   return ls.finish("kv_append");
-}
-
-extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const void* q, int64_t ld_q,
-                                  void* out, int64_t ld_out, int64_t max_q, float divisor, float softcap,
-                                  int64_t window, int64_t shared) {
-  int rc = enter(ctx);
-  if (rc) return rc;
-  PagedAttn p;
-  rc = paged_batch(ctx, desc, &p.b);
-  if (rc) return rc;
-  TL_REQUIRE(divisor > 0.f && divisor < INFINITY, "divisor must be positive and finite");
-  TL_REQUIRE(softcap >= 0.f && softcap < INFINITY, "softcap must be 0 or positive and finite");
-  TL_REQUIRE(max_q > 0, "max_q must be positive");
-  TL_REQUIRE(window >= 0, "negative window");
-  TL_REQUIRE(shared >= 0 && shared % desc->page_size == 0 && shared <= desc->table_cols * desc->page_size,
-             "shared must be whole pages of the table");
-  TL_REQUIRE(shared == 0 || window == 0, "a window and a shared prefix exclude each other");
-  if (desc->n_rows == 0 || desc->n_seqs == 0) return TL_OK;
-  const int64_t D = desc->head_dim, wq = desc->n_heads_q * D;
-  rc = check_rows(desc, q, ld_q, wq, "q");
-  if (rc) return rc;
-  rc = check_rows(desc, out, ld_out, wq, "out");
-  if (rc) return rc;
-  p.q = q; p.k = desc->k_pages; p.v = desc->v_pages; p.out = out;
-  p.ld_q = ld_q; p.ld_out = ld_out;
-  p.max_q = (int)std::min<int64_t>(max_q, desc->n_rows);
-  p.window = (int)std::min<int64_t>(window, 1LL << 30);
-  p.shared = (int)shared;
-  p.divisor = divisor; p.cap = softcap;
-  const double es = (double)dtype_size(desc->dtype);
-  // lengths are known on the device only: the profiler is told of the queries and outputs alone
-  LaunchScope ls(ctx, TL_KF_ATTENTION, 0, 2.0 * es * desc->n_rows * wq);
-  const unsigned grid = (unsigned)(desc->n_rows * desc->n_heads_q);
-  for_head_dim(D, [&](auto dim) {
-    constexpr int DD = decltype(dim)::value;
-    if (desc->dtype == TL_F32) paged_attention_simple_kernel<float, DD><<<grid, 64, 0, ctx->stream>>>(p);
-    else paged_attention_simple_kernel<bf16_t, DD><<<grid, 64, 0, ctx->stream>>>(p);
-  });
-  return ls.finish("paged_attention");
 }
 
 extern "C" int tl_i32_add(tl_ctx* ctx, int32_t* x, int64_t n, int32_t delta) {

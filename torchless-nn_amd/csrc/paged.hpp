@@ -55,7 +55,43 @@ __device__ __forceinline__ void check_shared(const PagedBatch& b, int s, const P
   if (__any(bad) && lane == 0) latch(b.status, kBadShare);
 }
 
+// The sequence that row t belongs to, by a whole wave: the last s with q_start[s] <= t, found by
+// 64 probes a round (one round up to 64 sequences, two up to 4096). n_seqs for a row of none.
+__device__ __forceinline__ int seq_of_row(const PagedBatch& b, int t, int lane) {
+  int lo = 0, n = b.n_seqs;  // q_start[lo] <= t as far as probed; the answer is in [lo, lo + n)
+  int hits = 0;
+  while (true) {
+    const int step = (n + 63) >> 6;
+    const int at = lo + (lane + 1) * step;
+    const bool hit = at <= lo + n && at <= b.n_seqs && b.q_start[at] <= t;
+    hits = __popcll(__ballot(hit));
+    if (step == 1) break;
+    lo += hits * step;
+    n = min(step, b.n_seqs - lo);
+    if (n <= 0) break;
+  }
+  return min(lo + (n > 0 ? hits : 0), b.n_seqs);
+}
+
 // Checks a descriptor and turns it into the kernels' form.
 int paged_batch(tl_ctx* ctx, const tl_paged_desc* d, PagedBatch* b);
+// Checks a tensor of the batch's rows: 16-byte aligned rows that do not overlap.
+int paged_rows(const tl_paged_desc* d, const void* p, int64_t ld, int64_t cols, const char* what);
+
+// Calls f with a D of the descriptor's head_dim as a type.
+template <int D>
+struct HeadDim {
+  static constexpr int value = D;
+};
+template <typename F>
+static void for_head_dim(int64_t d, F f) {
+  switch (d) {
+    case 32: f(HeadDim<32>{}); break;
+    case 64: f(HeadDim<64>{}); break;
+    case 128: f(HeadDim<128>{}); break;
+    default: f(HeadDim<256>{}); break;
+  }
+}
+
 
 }  // namespace tl

@@ -1,0 +1,710 @@
+// Causal attention of a ragged batch over a paged KV cache (keys and values [page, kv head, slot, D],
+// both row-major): the step kernel for batches of few rows a sequence, and the join of its parts.
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace tl {
+
+struct PagedAttn {
+  PagedBatch b;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t ld_q, ld_out;
+  int max_q, window;  // window 0: none
+  int shared, skip;   // positions that the sequences share, and those of them that another kernel takes
+  float scale;                // scores to log2 units: log2(e) / divisor, and with a cap
+  float cap_in, cap;          // 2 log2(e) / (divisor softcap) and log2(e) softcap; cap 0: none
+  // the step kernel's parts, [slot][group rows]: outputs [D] and (max, sum)
+  float* part_o;
+  float2* part_ml;
+  int workers;
+};
+
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const void* uniform(const void* p) {
+  const uint64_t x = (uint64_t)(uintptr_t)p;
+  return (const void*)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
+}
+__device__ __forceinline__ ConstInts const_ints(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
+
+// ---------------------------------------------------------------------------------------
+// keys and values in LDS
+// ---------------------------------------------------------------------------------------
+// Rows of a chunk lie in LDS one after another as 16-byte pieces. The pieces of a row are permuted by
+// an XOR with a number made from the row (applied to the source address of the direct load, which
+// writes linearly), so that the lanes that read LDS together meet different banks:
+//   keys: 16 lanes read the same piece of 16 rows;
+//   values (bf16): 16 lanes read 32 bytes of each of 4 rows, transposed; two such groups a phase.
+template <typename T, int D>
+struct Rows {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  static constexpr int kPieces = D / kVec;        // of a row
+  static constexpr int kBytes = D * (int)sizeof(T);
+  static constexpr int kPerLoad = 64 / kPieces;   // rows that one direct load of a wave covers
+  static_assert(kPieces <= 64 && kPerLoad <= 16, "row size");
+  __device__ __forceinline__ static int key_swizzle(int row) {
+    return kPieces >= 16 ? row & 15 : (row / (16 / kPieces)) & (kPieces - 1);
+  }
+  __device__ __forceinline__ static int value_swizzle(int row) {
+    constexpr int kSegs = kPieces / 2;  // of 32 bytes
+    if (sizeof(T) == 4) return 0;
+    return 2 * (kSegs >= 8 ? row & 7 : (row / (8 / (kSegs < 8 ? kSegs : 8))) & (kSegs - 1));
+  }
+};
+
+// dma_load16 from a uniform base and a per-lane byte offset.
+__device__ __forceinline__ void dma_load16_at(const void* base, uint32_t offset, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds), "v"(offset), "s"(base)
+      : "memory");
+}
+// Waits until at most n direct loads of the wave are in flight (n is uniform, a multiple of STEP).
+template <int STEP, int MOST>
+__device__ __forceinline__ void wait_loads(int n) {
+  if constexpr (MOST == 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  } else {
+    if (n >= MOST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MOST) : "memory");
+    else wait_loads<STEP, MOST - STEP>(n);
+  }
+}
+
+// Queues the 16 rows of one 16-position block of a page (uniform address) to LDS.
+template <typename T, int D, bool KEYS>
+__device__ __forceinline__ void load_block16(const void* src, uint32_t lds, int lane) {
+  using R = Rows<T, D>;
+  const int rr = lane / R::kPieces, c = lane % R::kPieces;
+#pragma unroll
+  for (int i = 0; i < 16 / R::kPerLoad; ++i) {
+    const int row = i * R::kPerLoad + rr;
+    const int sw = KEYS ? R::key_swizzle(row) : R::value_swizzle(row);
+    dma_load16_at(src, (uint32_t)(row * R::kBytes + ((c ^ sw) << 4)), lds + i * 1024);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// tile arithmetic: 16 rows of queries (columns of S^T and O^T) by 16-key tiles
+// ---------------------------------------------------------------------------------------
+// S^T = K Q^T: lane l of the wave holds the scores of query row l % 16 at keys 16 j + 4 (l / 16) + r.
+// O^T += V^T P^T takes those probabilities as its B operand where they are: bf16, 32 keys a step, in
+// the key order that the lanes hold; fp32, 4 keys a step, one of each lane group.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int D>
+struct Tile16 {
+  using R = Rows<T, D>;
+  static constexpr bool kBf = sizeof(T) == 2;
+  static constexpr int KS = R::kPieces / 4;          // steps of 4 pieces over D
+  static constexpr int DT = D / 16;                  // output tiles
+  static constexpr int E = DT < 4 ? DT : 4;          // fp32: consecutive outputs that one read feeds
+  using QFrag = uint4;
+
+  // 16 keys from row `row0` of a chunk against the wave's queries
+  __device__ __forceinline__ static f32x4 scores(const unsigned char* keys, int row0, const uint4* q, int fr, int fg) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    const int row = row0 + fr, sw = R::key_swizzle(row);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + row * R::kBytes + (((4 * ks + fg) ^ sw) << 4));
+      if constexpr (kBf) {
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q[ks]),
+                                                    s, 0, 0, 0);
+      } else {
+        const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[ks]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], s, 0, 0, 0);
+      }
+    }
+    return s;
+  }
+  // The bf16 operand V^T[16 t .. +15][32 keys] of keys 4 fg .. +3 and 16 + 4 fg .. +3 of `half`
+  __device__ __forceinline__ static bf16x8 value_frag(const unsigned char* values, int half, int t, int lane) {
+    const int sub = lane & 15, row = 32 * half + 4 * (lane >> 4) + (sub >> 2);
+    const int piece = 2 * t + ((sub >> 1) & 1), at = (sub & 1) * 8;
+    const unsigned char* lo = values + row * R::kBytes + ((piece ^ R::value_swizzle(row)) << 4) + at;
+    const unsigned char* hi = values + (row + 16) * R::kBytes + ((piece ^ R::value_swizzle(row + 16)) << 4) + at;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+    return __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // O^T += V^T P^T over KT tiles of 16 keys
+  template <int KT>
+  __device__ __forceinline__ static void values(const unsigned char* vals, const f32x4* s, f32x4* o, int lane) {
+    if constexpr (kBf) {
+#pragma unroll
+      for (int c = 0; c < KT / 2; ++c) {
+        bf16x8 pf;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          pf[r] = (__bf16)s[2 * c][r];
+          pf[4 + r] = (__bf16)s[2 * c + 1][r];
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_frag(vals, c, t, lane), pf, o[t], 0, 0, 0);
+      }
+    } else {
+      const int fr = lane & 15, fg = lane >> 4;
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const unsigned char* row = vals + (16 * j + 4 * fg + r) * R::kBytes + fr * (4 * E);
+#pragma unroll
+          for (int t = 0; t < DT / E; ++t) {
+            float a[E];
+            if constexpr (E == 4) *reinterpret_cast<f32x4*>(a) = *reinterpret_cast<const f32x4*>(row + t * 64 * E);
+            else *reinterpret_cast<f32x2*>(a) = *reinterpret_cast<const f32x2*>(row + t * 64 * E);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              o[t * E + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], s[j][r], o[t * E + e], 0, 0, 0);
+          }
+        }
+    }
+  }
+  // Calls f(d, x) for runs of 4 consecutive outputs x of the lane's query row, at d .. d + 3 (fp32 at
+  // D = 32: 2 runs of 4 all the same).
+  template <typename F>
+  __device__ __forceinline__ static void each_run(const f32x4* o, int fg, F f) {
+    if constexpr (kBf) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) f(16 * t + 4 * fg, o[t]);
+    } else if constexpr (E == 4) {
+#pragma unroll
+      for (int t = 0; t < DT / 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          f(64 * t + 16 * fg + 4 * r, f32x4{o[4 * t][r], o[4 * t + 1][r], o[4 * t + 2][r], o[4 * t + 3][r]});
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) f(8 * fg + 2 * r, f32x4{o[0][r], o[1][r], o[0][r + 1], o[1][r + 1]});
+    }
+  }
+};
+
+__device__ __forceinline__ void store_run(float* p, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ void store_run(bf16_t* p, f32x4 x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)f2bf(x[0]) | ((uint32_t)f2bf(x[1]) << 16),
+                                            (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16));
+}
+
+// A score in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), whose error of an fp32
+// rounding of c is far below bf16's steps; fp32 takes the library's tanh.
+template <typename T, bool CAP>
+__device__ __forceinline__ float score(const PagedAttn& p, float s) {
+  if constexpr (!CAP) return s * p.scale;
+  if constexpr (sizeof(T) == 4) return p.cap * tanhf(s * p.cap_in * 0.34657359027997264f);
+  const float e = __builtin_amdgcn_exp2f(s * p.cap_in);
+  return __builtin_fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(1.f + e), p.cap);
+}
+
+// ---------------------------------------------------------------------------------------
+// the step kernel
+// ---------------------------------------------------------------------------------------
+// Few rows a sequence (at most 16 of a kv head's query heads together): every key and value is read
+// once and used by one MFMA operand, so memory is the bound. The keys of all sequences and kv heads,
+// in chunks of KC, are one line that is cut into equal runs, one for each wave of the chip (a
+// workgroup), whatever the sequences' lengths are; a wave streams its run through an LDS ring of its
+// own (ST chunks, direct loads, no barrier), across the sequences' borders. A (sequence, kv head)
+// inside one run is finished there; the parts of one that is cut are joined by the second kernel.
+
+// What a sequence's rows see: positions lo .. hi - 1, row i those up to base + i.
+struct StepSeq {
+  int row0, n, base, lo, hi;
+};
+__device__ __forceinline__ StepSeq step_seq(const PagedAttn& p, int row0, int n, int len) {
+  StepSeq s;
+  s.row0 = row0;
+  s.n = min(n, p.max_q);
+  s.base = len - n;
+  s.lo = max(p.skip, p.window > 0 ? s.base - p.window + 1 : 0);
+  s.hi = s.base + s.n;
+  if (s.n <= 0 || s.hi <= s.lo) s.lo = s.hi = 0;
+  return s;
+}
+template <int KC>
+__device__ __forceinline__ int step_chunks(const StepSeq& s) {
+  return s.hi > 0 ? (s.hi + KC - 1) / KC - s.lo / KC : 0;
+}
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// The sequence at which a wave stands (uniform): read through the scalar cache, whose waits leave the
+// direct loads alone.
+__device__ __forceinline__ StepSeq step_seq_at(const PagedAttn& p, int s) {
+  ConstInts start = const_ints(p.b.q_start), len = const_ints(p.b.kv_len);
+  const int a = uniform(start[s]), e = uniform(start[s + 1]), l = uniform(len[s]);
+  const int row0 = min(max(a, 0), p.b.n_rows);
+  return step_seq(p, row0, min(max(e, row0), p.b.n_rows) - row0, min(max(l, 0), p.b.cols << p.b.page_shift));
+}
+
+template <int KC>
+struct StepCursor {
+  int s, h, c;  // sequence, kv head, chunk
+  StepSeq q;
+  __device__ __forceinline__ void next(const PagedAttn& p) {
+    if (++c < (q.hi + KC - 1) / KC) return;
+    if (++h == p.b.Hkv) {
+      h = 0;
+      do {
+        if (++s >= p.b.n_seqs) return;
+        q = step_seq_at(p, s);
+      } while (q.hi == 0);
+    }
+    c = q.lo / KC;
+  }
+};
+
+template <typename T, int D, int KC, int ST, bool CAP>
+__global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
+  using R = Rows<T, D>;
+  using M = Tile16<T, D>;
+  constexpr int KT = KC / 16, kHalf = KC * R::kBytes, kStage = 2 * kHalf;
+  constexpr int kLoads = kHalf / 1024;  // direct loads for a chunk's keys, and for its values
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[ST * kStage];
+  const int lane = threadIdx.x, fr = lane & 15, fg = lane >> 4;
+  const int w = blockIdx.x, g = p.b.Hq / p.b.Hkv;
+
+  // this wave's run [begin, end) of the line of chunks, and where it begins
+  int total = 0, mine = 0;
+  for (int s = lane; s < p.b.n_seqs; s += 64) {
+    const PagedSeq q = paged_seq(p.b, s, false);
+    mine = step_chunks<KC>(step_seq(p, q.row0, q.n, q.len));
+    total += mine;
+  }
+  total = uniform(wave_sum_int(total) * p.b.Hkv);
+  const int per = (int)(((uint32_t)total + p.workers - 1) / (uint32_t)p.workers);
+  const int begin = uniform(w * per), end = min(total, begin + uniform(per));
+  if (begin >= end) return;
+  StepCursor<KC> ld;
+  {
+    int before = 0, s0 = 0, incl;
+    while (true) {
+      if (p.b.n_seqs > 64) {
+        mine = 0;
+        if (s0 + lane < p.b.n_seqs) {
+          const PagedSeq q = paged_seq(p.b, s0 + lane, false);
+          mine = step_chunks<KC>(step_seq(p, q.row0, q.n, q.len));
+        }
+      }
+      incl = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
+      }
+      const uint64_t past = __ballot((before + incl) * p.b.Hkv > begin);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        ld.s = uniform(s0 + at);
+        before = uniform(before + __shfl(incl - mine, at, 64));
+        mine = uniform(__shfl(mine, at, 64));
+        break;
+      }
+      before += uniform(__shfl(incl, 63, 64));
+      s0 += 64;
+      if (s0 >= p.b.n_seqs) return;  // not reached: begin < total
+    }
+    ld.q = step_seq_at(p, ld.s);
+    const int off = begin - before * p.b.Hkv;
+    ld.h = uniform(off / mine);
+    ld.c = uniform(ld.q.lo / KC + off % mine);
+  }
+  StepCursor<KC> cp = ld;
+
+  const uint32_t ring0 = lds_offset(ring);
+  auto issue = [&](int stage) {
+    const int k0 = ld.c * KC;
+    ConstInts row = const_ints(p.b.table) + (int64_t)ld.s * p.b.ld_table;
+    int id[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      // a block without a visible position is read from page 0: its scores are masked, its values zeroed
+      const int pos = k0 + 16 * j;
+      const bool use = pos < ld.q.hi && pos + 16 > ld.q.lo;
+      const int x = uniform(row[min(pos >> p.b.page_shift, p.b.cols - 1)]);
+      const bool ok = (uint32_t)x < (uint32_t)p.b.n_pages;
+      if (use && !ok && lane == 0) latch(p.b.status, kBadPage);
+      id[j] = use && ok ? x : 0;
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const unsigned char* base = (const unsigned char*)(v ? p.v : p.k);
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        const int slot = (k0 + 16 * j) & ((1 << p.b.page_shift) - 1);
+        const unsigned char* src = base + ((((int64_t)id[j] * p.b.Hkv + ld.h) << p.b.page_shift) + slot) * R::kBytes;
+        const int lds = (int)ring0 + stage * kStage + v * kHalf + j * 16 * R::kBytes;
+        if (v) load_block16<T, D, false>(uniform(src), uniform(lds), lane);
+        else load_block16<T, D, true>(uniform(src), uniform(lds), lane);
+      }
+    }
+  };
+
+  const int count = end - begin;
+  int queued = 0;
+#pragma unroll
+  for (int st = 0; st < ST; ++st)
+    if (queued < count) {
+      issue(st);
+      ld.next(p);
+      ++queued;
+    }
+
+  uint4 qf[M::KS];
+  f32x4 o[M::DT];
+  float m_run = -INFINITY, l_part = 0.f;
+  bool fresh = true, first_item = true;
+  int c_first = cp.c, stage = 0, token = 0, head = 0;
+  for (int it = 0; it < count; ++it) {
+    if (fresh) {
+      // rows of the item: token fr / g, query head fr % g of the kv head's; the columns past them repeat the first
+      const bool row_ok = fr < cp.q.n * g;
+      token = row_ok ? fr / g : 0;
+      head = cp.h * g + (row_ok ? fr - token * g : 0);
+      const T* qr = (const T*)p.q + (int64_t)(cp.q.row0 + token) * p.ld_q + head * D;
+#pragma unroll
+      for (int ks = 0; ks < M::KS; ++ks) qf[ks] = *reinterpret_cast<const uint4*>(qr + (4 * ks + fg) * R::kVec);
+      // waited for here, once an item: at their first use the compiler would wait in every chunk, for the
+      // direct loads in flight too
+#pragma unroll
+      for (int ks = 0; ks < M::KS; ++ks) asm volatile("" : "+v"(qf[ks].x), "+v"(qf[ks].y), "+v"(qf[ks].z), "+v"(qf[ks].w));
+#pragma unroll
+      for (int t = 0; t < M::DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run = -INFINITY;
+      l_part = 0.f;
+      c_first = cp.c;
+      fresh = false;
+    }
+    const int ahead = (queued - it - 1) * 2 * kLoads;  // loads queued after this chunk's
+    const unsigned char* keys = ring + stage * kStage;
+    unsigned char* vals = ring + stage * kStage + kHalf;
+    wait_loads<kLoads, (2 * ST - 1) * kLoads>(ahead + kLoads);
+    f32x4 s[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) s[j] = M::scores(keys, 16 * j, qf, fr, fg);
+
+    const int k0 = cp.c * KC;
+    const int pos = cp.q.base + token;
+    const int lo = max(p.skip, p.window > 0 ? pos - p.window + 1 : 0);
+    const bool whole = k0 >= max(p.skip, p.window > 0 ? cp.q.hi - p.window : 0) && k0 + KC <= cp.q.base + 1;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[j][r] = score<T, CAP>(p, s[j][r]);
+        if (!whole) {
+          const int key = k0 + 16 * j + 4 * fg + r;
+          s[j][r] = key >= lo && key <= pos ? s[j][r] : -INFINITY;
+        }
+        mx = fmaxf(mx, s[j][r]);
+      }
+    // the reference maximum moves only when a score passes it by more than 2^8, and only then the
+    // row's four lanes are asked (unnormalised probabilities stay below 2^8)
+    if (__any(mx > m_run + 8.f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = mx > m_run + 8.f ? mx : m_run;
+      const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_part *= alpha;
+#pragma unroll
+      for (int t = 0; t < M::DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[t][r] *= alpha;
+      m_run = m_new;
+    }
+    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - m_ref);
+        l_part += s[j][r];
+      }
+    wait_loads<kLoads, (2 * ST - 2) * kLoads>(ahead);
+    if (k0 < cp.q.lo || k0 + KC > cp.q.hi) {
+      // positions that no row sees may hold anything, and 0 times a NaN would be one
+      for (int x = lane; x < KC * R::kPieces; x += 64) {
+        const int key = k0 + x / R::kPieces;
+        if (key < cp.q.lo || key >= cp.q.hi) *reinterpret_cast<uint4*>(vals + x * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    M::template values<KT>(vals, s, o, lane);
+    // the stage is free once its reads have returned
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (queued < count) {
+      issue(stage);
+      ld.next(p);
+      ++queued;
+    }
+    stage = stage + 1 == ST ? 0 : stage + 1;
+
+    const bool last = cp.c + 1 == (cp.q.hi + KC - 1) / KC;
+    if (last || it + 1 == count) {
+      float l = l_part + __shfl_xor(l_part, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      const bool all = last && c_first == cp.q.lo / KC;
+      if (fr < cp.q.n * g) {
+        if (all) {
+          T* orow = (T*)p.out + (int64_t)(cp.q.row0 + token) * p.ld_out + head * D;
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          M::each_run(o, fg, [&](int d, f32x4 x) { store_run(orow + d, x * inv); });
+        } else {
+          // a run has at most two items that it does not hold whole: the one it begins in, and its last
+          const int64_t slot = (int64_t)(2 * w + (first_item ? 0 : 1)) * (p.max_q * g) + fr;
+          float* orow = p.part_o + slot * D;
+          M::each_run(o, fg, [&](int d, f32x4 x) { store_run(orow + d, x); });
+          if (fg == 0) p.part_ml[slot] = make_float2(m_run, l);
+        }
+      }
+      fresh = true;
+      first_item = false;
+    }
+    cp.next(p);
+  }
+}
+
+// Joins the parts of one (row, query head): out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m the
+// largest m_i. Also what the step kernel has no chunk for: zeros for rows that see nothing, and the
+// report of bounds that are out of range. Every workgroup finds its parts from the lengths, as the
+// step kernel found its runs; the parts are taken in their order, so results repeat bit for bit.
+template <typename T, int D, int KC>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads of a part, parts at a time
+  __shared__ int sums[4][2];
+  __shared__ f32x4 acc[kGroups][kLanes];
+  __shared__ float lsum[kGroups];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int t = blockIdx.x / p.b.Hq, head = blockIdx.x - t * p.b.Hq, g = p.b.Hq / p.b.Hkv;
+  const int sq = seq_of_row(p.b, t, lane);
+  if (sq >= p.b.n_seqs) return;
+  const PagedSeq raw = paged_seq(p.b, sq, head == 0 && tid == 0);
+  const StepSeq q = step_seq(p, raw.row0, raw.n, raw.len);
+  const int i = t - raw.row0;
+  if (i < 0 || i >= raw.n) return;
+  if (head == 0 && i == 0 && wave == 0 && p.shared > 0) check_shared(p.b, sq, raw, p.shared, lane);
+  if (i >= q.n) {
+    if (tid == 0) latch(p.b.status, kBadSequence);
+    return;
+  }
+  T* orow = (T*)p.out + (int64_t)t * p.ld_out + head * D;
+  const int chunks = step_chunks<KC>(q);
+  int all = 0, before = 0;
+  for (int s = tid; s < p.b.n_seqs; s += 256) {
+    const PagedSeq x = paged_seq(p.b, s, false);
+    const int c = step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
+    all += c;
+    before += s < sq ? c : 0;
+  }
+  all = wave_sum_int(all);
+  before = wave_sum_int(before);
+  if (lane == 0) {
+    sums[wave][0] = all;
+    sums[wave][1] = before;
+  }
+  __syncthreads();
+  all = (sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0]) * p.b.Hkv;
+  before = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
+  if (chunks == 0) {
+    if (tid < kLanes) store_run(orow + 4 * tid, f32x4{0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  const int per = (int)(((uint32_t)all + p.workers - 1) / (uint32_t)p.workers);
+  const int a = before * p.b.Hkv + (head / g) * chunks;
+  const int wa = a / per, parts = (a + chunks - 1) / per - wa + 1;
+  if (parts == 1) return;  // finished by the step kernel
+  const int rows = p.max_q * g, row = i * g + head % g;
+  auto slot = [&](int k) -> int64_t {
+    return (int64_t)(2 * (wa + k) + (k > 0 || a == wa * per ? 0 : 1)) * rows + row;
+  };
+  float m = -INFINITY;
+  for (int k = lane; k < parts; k += 64) m = fmaxf(m, p.part_ml[slot(k)].x);
+  m = wave_max(m);
+  if (m == -INFINITY) m = 0.f;
+  const int grp = tid / kLanes, at = tid % kLanes;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int k = grp; k < parts; k += kGroups) {
+    const int64_t s = slot(k);
+    const float2 ml = p.part_ml[s];
+    const float e = __builtin_amdgcn_exp2f(ml.x - m);
+    l += e * ml.y;
+    o += e * *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * at);
+  }
+  acc[grp][at] = o;
+  if (at == 0) lsum[grp] = l;
+  __syncthreads();
+  if (tid < kLanes) {
+    for (int k = 1; k < kGroups; ++k) {
+      o += acc[k][tid];
+      l += lsum[k];
+    }
+    store_run(orow + 4 * tid, o * (l > 0.f ? 1.f / l : 0.f));
+  }
+}
+
+// One wave per (row, query head): each lane takes a key of 64, then an element of the output.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void paged_attention_simple_kernel(PagedAttn p) {
+  __shared__ float qs[D];
+  const int lane = threadIdx.x;
+  const int t = blockIdx.x / p.b.Hq, h = blockIdx.x % p.b.Hq;
+  const int s = seq_of_row(p.b, t, lane);
+  if (s >= p.b.n_seqs) return;
+  const PagedSeq q = paged_seq(p.b, s, lane == 0);
+  const int i = t - q.row0;
+  if (i < 0 || i >= q.n) return;
+  if (p.shared > 0) check_shared(p.b, s, q, p.shared, lane);
+  if (i >= p.max_q) {
+    if (lane == 0) latch(p.b.status, kBadSequence);
+    return;
+  }
+  const int pos = q.len - q.n + i;
+  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int32_t* row = p.b.table + s * p.b.ld_table;
+  const T* qr = (const T*)p.q + t * p.ld_q + h * D;
+  for (int d = lane; d < D; d += 64) qs[d] = Elem<T>::load(qr + d);
+  __syncthreads();
+  const int hk = h / (p.b.Hq / p.b.Hkv), mask = (1 << p.b.page_shift) - 1;
+  constexpr int E = (D + 63) / 64;
+  float o[E] = {}, m = -INFINITY, l = 0.f;
+  for (int j0 = first; j0 <= pos; j0 += 64) {
+    const int j = j0 + lane;
+    float sc = -INFINITY;
+    int64_t at = 0;
+    if (j <= pos) {
+      const int64_t page = paged_page(p.b, row, j, true);
+      at = (((page * p.b.Hkv + hk) << p.b.page_shift) + (j & mask)) * D;
+      float a = 0.f;
+      for (int d = 0; d < D; ++d) a += qs[d] * Elem<T>::load((const T*)p.k + at + d);
+      sc = a * p.scale * 0.6931471805599453f;
+      if (p.cap > 0.f) sc = 0.6931471805599453f * p.cap * tanhf(a * p.cap_in * 0.34657359027997264f);
+    }
+    const float mn = fmaxf(m, wave_max(sc));
+    const float e = expf(sc - mn), al = expf(m - mn);
+    l = l * al + wave_sum(e);
+    m = mn;
+#pragma unroll
+    for (int x = 0; x < E; ++x) o[x] *= al;
+    const int n = min(64, pos + 1 - j0);
+    for (int y = 0; y < n; ++y) {
+      const float w = __shfl(e, y, 64);
+      const int64_t a = (int64_t)__shfl((long long)at, y, 64);
+#pragma unroll
+      for (int x = 0; x < E; ++x)
+        if (x * 64 + lane < D) o[x] += w * Elem<T>::load((const T*)p.v + a + x * 64 + lane);
+    }
+  }
+  T* orow = (T*)p.out + t * p.ld_out + h * D;
+#pragma unroll
+  for (int x = 0; x < E; ++x)
+    if (x * 64 + lane < D) Elem<T>::store(orow + x * 64 + lane, l > 0.f ? o[x] / l : 0.f);
+}
+
+
+// ---------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------
+// Chunks and ring of the step kernel: 16 KB of keys and values a chunk (32 KB at the widest rows), as many
+// waves on a CU as its 160 KB of LDS hold.
+template <typename T, int D>
+struct StepShape {
+  static constexpr int kRow = D * (int)sizeof(T);
+  static constexpr int KC = kRow <= 128 ? 64 : kRow <= 512 ? 32 : 16;
+  static constexpr int ST = kRow * KC * 2 > 16384 ? 2 : 3;
+  static constexpr int kLds = ST * 2 * KC * kRow;
+  static constexpr int kPerCu = (160 * 1024) / kLds < 8 ? (160 * 1024) / kLds : 8;
+};
+
+template <typename T, int D>
+static int launch_step(tl_ctx* ctx, PagedAttn p) {
+  using S = StepShape<T, D>;
+  const int64_t rows = (int64_t)p.max_q * (p.b.Hq / p.b.Hkv);
+  const int64_t most = (int64_t)p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
+  TL_REQUIRE(most < (1LL << 30), "batch too large: sequences x kv heads x table positions");
+  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)S::kPerCu * (ctx->num_cus > 0 ? ctx->num_cus : 256)));
+  const size_t obytes = (size_t)p.workers * 2 * rows * D * sizeof(float);
+  void* ws;
+  const int rc = workspace(ctx, obytes + (size_t)p.workers * 2 * rows * sizeof(float2), &ws);
+  if (rc) return rc;
+  p.part_o = (float*)ws;
+  p.part_ml = (float2*)((char*)ws + obytes);
+  if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
+  else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
+  paged_join_kernel<T, D, S::KC><<<(unsigned)(p.b.n_rows * p.b.Hq), 256, 0, ctx->stream>>>(p);
+  return TL_OK;
+}
+
+template <typename T, int D>
+static int launch_attention(tl_ctx* ctx, PagedAttn p) {
+  const int64_t g = p.b.Hq / p.b.Hkv;
+  if (p.max_q * g <= 16) {
+    p.skip = 0;
+    return launch_step<T, D>(ctx, p);
+  }
+  paged_attention_simple_kernel<T, D><<<(unsigned)(p.b.n_rows * p.b.Hq), 64, 0, ctx->stream>>>(p);
+  return TL_OK;
+}
+
+}  // namespace tl
+
+using namespace tl;
+
+extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const void* q, int64_t ld_q,
+                                  void* out, int64_t ld_out, int64_t max_q, float divisor, float softcap,
+                                  int64_t window, int64_t shared) {
+  int rc = enter(ctx);
+  if (rc) return rc;
+  PagedAttn p;
+  rc = paged_batch(ctx, desc, &p.b);
+  if (rc) return rc;
+  TL_REQUIRE(divisor > 0.f && divisor < INFINITY, "divisor must be positive and finite");
+  TL_REQUIRE(softcap >= 0.f && softcap < INFINITY, "softcap must be 0 or positive and finite");
+  TL_REQUIRE(max_q > 0, "max_q must be positive");
+  TL_REQUIRE(window >= 0, "negative window");
+  TL_REQUIRE(shared >= 0 && shared % desc->page_size == 0 && shared <= desc->table_cols * desc->page_size,
+             "shared must be whole pages of the table");
+  TL_REQUIRE(shared == 0 || window == 0, "a window and a shared prefix exclude each other");
+  if (desc->n_rows == 0 || desc->n_seqs == 0) return TL_OK;
+  const int64_t D = desc->head_dim, wq = desc->n_heads_q * D;
+  rc = paged_rows(desc, q, ld_q, wq, "q");
+  if (rc) return rc;
+  rc = paged_rows(desc, out, ld_out, wq, "out");
+  if (rc) return rc;
+  p.q = q; p.k = desc->k_pages; p.v = desc->v_pages; p.out = out;
+  p.ld_q = ld_q; p.ld_out = ld_out;
+  p.max_q = (int)std::min<int64_t>(max_q, desc->n_rows);
+  p.window = (int)std::min<int64_t>(window, 1LL << 30);
+  p.shared = (int)shared;
+  const double log2e = 1.4426950408889634;
+  p.scale = (float)(log2e / divisor);
+  p.cap_in = softcap > 0.f ? (float)(2.0 * log2e / ((double)divisor * softcap)) : 0.f;
+  p.cap = (float)(log2e * softcap);
+  p.part_o = nullptr; p.part_ml = nullptr; p.workers = 0;
+  const double es = (double)dtype_size(desc->dtype);
+  // lengths are known on the device only: the profiler is told of the queries and outputs alone
+  LaunchScope ls(ctx, TL_KF_ATTENTION, 0, 2.0 * es * desc->n_rows * wq);
+  rc = TL_OK;
+  for_head_dim(D, [&](auto dim) {
+    constexpr int DD = decltype(dim)::value;
+    rc = desc->dtype == TL_F32 ? launch_attention<float, DD>(ctx, p) : launch_attention<bf16_t, DD>(ctx, p);
+  });
+  if (rc) return rc;
+  return ls.finish("paged_attention");
+}
