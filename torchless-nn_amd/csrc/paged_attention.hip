@@ -6,6 +6,12 @@
 
 namespace tl {
 
+// A block of a sequence's rows (row r: token r / g, query head r % g of the kv head's) and the chunks
+// that they see: chunk0 .. chunk0 + chunks - 1, which lie at `at` on the line.
+struct PagedTile {
+  int seq, row, chunk0, chunks, at;
+};
+
 struct PagedAttn {
   PagedBatch b;
   const void* q;
@@ -21,6 +27,9 @@ struct PagedAttn {
   float* part_o;
   float2* part_ml;
   int workers;
+  // the tile kernel's plan: row blocks of the batch, in order; per kv head they are one line of chunks
+  PagedTile* tiles;
+  int most_tiles;
 };
 
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;
@@ -109,25 +118,29 @@ struct Tile16 {
   static constexpr int KS = R::kPieces / 4;          // steps of 4 pieces over D
   static constexpr int DT = D / 16;                  // output tiles
   static constexpr int E = DT < 4 ? DT : 4;          // fp32: consecutive outputs that one read feeds
-  using QFrag = uint4;
 
-  // 16 keys from row `row0` of a chunk against the wave's queries
-  __device__ __forceinline__ static f32x4 scores(const unsigned char* keys, int row0, const uint4* q, int fr, int fg) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  // Scores of 16 keys from row `row0` of a chunk against RG groups of 16 queries (q[group][KS])
+  template <int RG>
+  __device__ __forceinline__ static void scores(const unsigned char* keys, int row0, const uint4* q, f32x4* s, int fr,
+                                                int fg) {
     const int row = row0 + fr, sw = R::key_swizzle(row);
+#pragma unroll
+    for (int i = 0; i < RG; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const uint4 k = *reinterpret_cast<const uint4*>(keys + row * R::kBytes + (((4 * ks + fg) ^ sw) << 4));
-      if constexpr (kBf) {
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q[ks]),
-                                                    s, 0, 0, 0);
-      } else {
-        const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[ks]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], s, 0, 0, 0);
+      for (int i = 0; i < RG; ++i) {
+        if constexpr (kBf) {
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
+                                                         __builtin_bit_cast(bf16x8, q[i * KS + ks]), s[i], 0, 0, 0);
+        } else {
+          const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[i * KS + ks]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], s[i], 0, 0, 0);
+        }
       }
     }
-    return s;
   }
   // The bf16 operand V^T[16 t .. +15][32 keys] of keys 4 fg .. +3 and 16 + 4 fg .. +3 of `half`
   __device__ __forceinline__ static bf16x8 value_frag(const unsigned char* values, int half, int t, int lane) {
@@ -139,21 +152,27 @@ struct Tile16 {
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
     return __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  // O^T += V^T P^T over KT tiles of 16 keys
-  template <int KT>
+  // O^T += V^T P^T over KT tiles of 16 keys: s[tile][group], o[group][DT]
+  template <int KT, int RG>
   __device__ __forceinline__ static void values(const unsigned char* vals, const f32x4* s, f32x4* o, int lane) {
     if constexpr (kBf) {
 #pragma unroll
       for (int c = 0; c < KT / 2; ++c) {
-        bf16x8 pf;
+        bf16x8 pf[RG];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          pf[r] = (__bf16)s[2 * c][r];
-          pf[4 + r] = (__bf16)s[2 * c + 1][r];
+        for (int i = 0; i < RG; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            pf[i][r] = (__bf16)s[2 * c * RG + i][r];
+            pf[i][4 + r] = (__bf16)s[(2 * c + 1) * RG + i][r];
+          }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const bf16x8 vf = value_frag(vals, c, t, lane);
+#pragma unroll
+          for (int i = 0; i < RG; ++i)
+            o[i * DT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[i], o[i * DT + t], 0, 0, 0);
         }
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_frag(vals, c, t, lane), pf, o[t], 0, 0, 0);
       }
     } else {
       const int fr = lane & 15, fg = lane >> 4;
@@ -168,8 +187,11 @@ struct Tile16 {
             if constexpr (E == 4) *reinterpret_cast<f32x4*>(a) = *reinterpret_cast<const f32x4*>(row + t * 64 * E);
             else *reinterpret_cast<f32x2*>(a) = *reinterpret_cast<const f32x2*>(row + t * 64 * E);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-              o[t * E + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], s[j][r], o[t * E + e], 0, 0, 0);
+            for (int i = 0; i < RG; ++i)
+#pragma unroll
+              for (int e = 0; e < E; ++e)
+                o[i * DT + t * E + e] =
+                    __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], s[j * RG + i][r], o[i * DT + t * E + e], 0, 0, 0);
           }
         }
     }
@@ -397,7 +419,7 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
     wait_loads<kLoads, (2 * ST - 1) * kLoads>(ahead + kLoads);
     f32x4 s[KT];
 #pragma unroll
-    for (int j = 0; j < KT; ++j) s[j] = M::scores(keys, 16 * j, qf, fr, fg);
+    for (int j = 0; j < KT; ++j) M::template scores<1>(keys, 16 * j, qf, s + j, fr, fg);
 
     const int k0 = cp.c * KC;
     const int pos = cp.q.base + token;
@@ -445,7 +467,7 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
         if (key < cp.q.lo || key >= cp.q.hi) *reinterpret_cast<uint4*>(vals + x * 16) = make_uint4(0, 0, 0, 0);
       }
     }
-    M::template values<KT>(vals, s, o, lane);
+    M::template values<KT, 1>(vals, s, o, lane);
     // the stage is free once its reads have returned
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (queued < count) {
@@ -559,64 +581,304 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   }
 }
 
-// One wave per (row, query head): each lane takes a key of 64, then an element of the output.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_attention_simple_kernel(PagedAttn p) {
-  __shared__ float qs[D];
-  const int lane = threadIdx.x;
-  const int t = blockIdx.x / p.b.Hq, h = blockIdx.x % p.b.Hq;
-  const int s = seq_of_row(p.b, t, lane);
-  if (s >= p.b.n_seqs) return;
-  const PagedSeq q = paged_seq(p.b, s, lane == 0);
-  const int i = t - q.row0;
-  if (i < 0 || i >= q.n) return;
-  if (p.shared > 0) check_shared(p.b, s, q, p.shared, lane);
-  if (i >= p.max_q) {
-    if (lane == 0) latch(p.b.status, kBadSequence);
-    return;
-  }
-  const int pos = q.len - q.n + i;
-  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  const int32_t* row = p.b.table + s * p.b.ld_table;
-  const T* qr = (const T*)p.q + t * p.ld_q + h * D;
-  for (int d = lane; d < D; d += 64) qs[d] = Elem<T>::load(qr + d);
+// ---------------------------------------------------------------------------------------
+// the tile kernel
+// ---------------------------------------------------------------------------------------
+// Prompts: blocks of NW x RG x 16 rows (tokens x the kv head's query heads, so that they share its keys
+// and values) against chunks of KC positions in LDS, double-buffered by direct loads. A plan made on the
+// device lists the blocks of all sequences and the chunks that each sees; per kv head they are one line,
+// the lines one after another, cut into equal runs for as many workgroups as are resident: neither
+// unequal lengths nor the causal triangle leave a workgroup idle. A block cut by a run's border leaves
+// parts, which a third launch joins.
+template <int BQ, int KC>
+__global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* total) {
+  __shared__ int wsum[16];
+  __shared__ int carry;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.b.Hq / p.b.Hkv;
+  // inclusive sum over the workgroup plus what went before; all threads call it
+  auto scan = [&](int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o, 64);
+      if (lane >= o) x += y;
+    }
+    if (lane == 63) wsum[wave] = x;
+    __syncthreads();
+    int add = carry, all = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      add += i < wave ? wsum[i] : 0;
+      all += wsum[i];
+    }
+    __syncthreads();
+    if (tid == 0) carry += all;
+    __syncthreads();
+    return x + add;
+  };
+  if (tid == 0) carry = 0;
   __syncthreads();
-  const int hk = h / (p.b.Hq / p.b.Hkv), mask = (1 << p.b.page_shift) - 1;
-  constexpr int E = (D + 63) / 64;
-  float o[E] = {}, m = -INFINITY, l = 0.f;
-  for (int j0 = first; j0 <= pos; j0 += 64) {
-    const int j = j0 + lane;
-    float sc = -INFINITY;
-    int64_t at = 0;
-    if (j <= pos) {
-      const int64_t page = paged_page(p.b, row, j, true);
-      at = (((page * p.b.Hkv + hk) << p.b.page_shift) + (j & mask)) * D;
-      float a = 0.f;
-      for (int d = 0; d < D; ++d) a += qs[d] * Elem<T>::load((const T*)p.k + at + d);
-      sc = a * p.scale * 0.6931471805599453f;
-      if (p.cap > 0.f) sc = 0.6931471805599453f * p.cap * tanhf(a * p.cap_in * 0.34657359027997264f);
+  // the first block of each sequence goes where it belongs in the list; the rest follow from it
+  int* first = total + 1;  // [n_seqs + 1]
+  for (int s0 = 0; s0 < p.b.n_seqs; s0 += 1024) {
+    const int s = s0 + tid;
+    int n = 0;
+    if (s < p.b.n_seqs) {
+      const PagedSeq q = paged_seq(p.b, s, true);
+      if (q.n > p.max_q) latch(p.b.status, kBadSequence);
+      n = (min(q.n, p.max_q) * g + BQ - 1) / BQ;
     }
-    const float mn = fmaxf(m, wave_max(sc));
-    const float e = expf(sc - mn), al = expf(m - mn);
-    l = l * al + wave_sum(e);
-    m = mn;
-#pragma unroll
-    for (int x = 0; x < E; ++x) o[x] *= al;
-    const int n = min(64, pos + 1 - j0);
-    for (int y = 0; y < n; ++y) {
-      const float w = __shfl(e, y, 64);
-      const int64_t a = (int64_t)__shfl((long long)at, y, 64);
-#pragma unroll
-      for (int x = 0; x < E; ++x)
-        if (x * 64 + lane < D) o[x] += w * Elem<T>::load((const T*)p.v + a + x * 64 + lane);
-    }
+    const int end = scan(n);
+    if (s < p.b.n_seqs) first[s] = end - n;
   }
-  T* orow = (T*)p.out + t * p.ld_out + h * D;
-#pragma unroll
-  for (int x = 0; x < E; ++x)
-    if (x * 64 + lane < D) Elem<T>::store(orow + x * 64 + lane, l > 0.f ? o[x] / l : 0.f);
+  const int tiles = min(carry, p.most_tiles);
+  __syncthreads();
+  if (tid == 0) {
+    first[p.b.n_seqs] = tiles;
+    carry = 0;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int t0 = 0; t0 < tiles; t0 += 1024) {
+    const int t = t0 + tid;
+    PagedTile x = {0, 0, 0, 0, 0};
+    if (t < tiles) {
+      int lo = 0, hi = p.b.n_seqs;  // the last s with first[s] <= t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const PagedSeq q = paged_seq(p.b, lo, false);
+      const int n = min(q.n, p.max_q), base = q.len - q.n;
+      x.seq = lo;
+      x.row = (t - first[lo]) * BQ;
+      const int a = max(0, p.window > 0 ? base + x.row / g - p.window + 1 : 0);
+      const int e = base + (min(x.row + BQ, n * g) - 1) / g + 1;
+      x.chunk0 = a / KC;
+      x.chunks = e > a ? (e + KC - 1) / KC - x.chunk0 : 0;
+    }
+    const int end = scan(x.chunks);
+    x.at = end - x.chunks;
+    if (t < tiles) p.tiles[t] = x;
+  }
+  if (tid == 0) *total = carry;
+  if (p.shared > 0)
+    for (int s = wave; s < p.b.n_seqs; s += 16) check_shared(p.b, s, paged_seq(p.b, s, false), p.shared, lane);
 }
 
+// Where on the lines a worker's run begins and ends: total chunks of a line, as equal runs as can be.
+__device__ __forceinline__ int tile_run(const PagedAttn& p, int line) {
+  return (int)(((uint32_t)line * p.b.Hkv + p.workers - 1) / (uint32_t)p.workers);
+}
+
+template <typename T, int D, int NW, int RG, int KC, bool CAP>
+__global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const int* total) {
+  using R = Rows<T, D>;
+  using M = Tile16<T, D>;
+  constexpr int KT = KC / 16, BQ = 16 * RG * NW, kHalf = KC * R::kBytes;
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[2][2 * kHalf];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), fr = lane & 15, fg = lane >> 4;
+  const int g = p.b.Hq / p.b.Hkv;
+  // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
+  const int w = (int)(blockIdx.x % 8) * (p.workers / 8) + (int)(blockIdx.x / 8);
+  const int line = total[0], tiles = total[1 + p.b.n_seqs];
+  const int per = tile_run(p, line);
+  int at = w * per;
+  const int stop = min(line * p.b.Hkv, at + per);
+  const uint32_t ring0 = lds_offset(ring);
+  bool first_item = true;
+  while (at < stop) {
+    const int h = at / line, off = at - h * line;
+    int lo = 0, hi = tiles;  // the last tile that starts at or before off and has chunks
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.tiles[mid].at <= off) lo = mid;
+      else hi = mid;
+    }
+    const PagedTile x = p.tiles[lo];
+    const int c0 = uniform(x.chunk0 + off - x.at), count = uniform(min(x.at + x.chunks - off, stop - at));
+    const int seq = uniform(x.seq);
+    const PagedSeq q = paged_seq(p.b, seq, false);
+    const int n = uniform(min(q.n, p.max_q) * g), base = uniform(q.len - q.n), row0 = uniform(x.row);
+    const int hi_pos = base + (min(row0 + BQ, n) - 1) / g + 1;
+    const int lo_pos = max(0, p.window > 0 ? base + row0 / g - p.window + 1 : 0);
+    const int32_t* pages = p.b.table + (int64_t)seq * p.b.ld_table;
+
+    auto issue = [&](int c, int stage) {
+#pragma unroll
+      for (int b = 0; b < 2 * KT; b += NW) {
+        const int blk = b + wave;  // keys' blocks, then values'
+        if (2 * KT % NW != 0 && blk >= 2 * KT) break;
+        const int j = blk % KT, pos = c * KC + 16 * j;
+        const bool use = pos < hi_pos && pos + 16 > lo_pos;
+        const int id = const_ints(pages)[min(pos >> p.b.page_shift, p.b.cols - 1)];
+        const bool ok = (uint32_t)id < (uint32_t)p.b.n_pages;
+        if (use && !ok && lane == 0) latch(p.b.status, kBadPage);
+        const int slot = pos & ((1 << p.b.page_shift) - 1);
+        const int64_t from = ((((int64_t)(use && ok ? id : 0) * p.b.Hkv + h) << p.b.page_shift) + slot) * R::kBytes;
+        const int lds = (int)ring0 + stage * 2 * kHalf + (blk / KT) * kHalf + j * 16 * R::kBytes;
+        if (blk < KT) load_block16<T, D, true>(uniform((const unsigned char*)p.k + from), uniform(lds), lane);
+        else load_block16<T, D, false>(uniform((const unsigned char*)p.v + from), uniform(lds), lane);
+      }
+    };
+    issue(c0, 0);
+
+    // this wave's rows
+    uint4 qf[RG * M::KS];
+    int pos_r[RG], lo_r[RG];
+    f32x4 o[RG * M::DT];
+    float m_run[RG], l_part[RG];
+    const int wrow = row0 + wave * 16 * RG;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+      const int r = min(wrow + 16 * i + fr, n - 1), token = r / g;
+      const T* qr = (const T*)p.q + (int64_t)(q.row0 + token) * p.ld_q + (h * g + r - token * g) * D;
+#pragma unroll
+      for (int ks = 0; ks < M::KS; ++ks)
+        qf[i * M::KS + ks] = *reinterpret_cast<const uint4*>(qr + (4 * ks + fg) * R::kVec);
+      pos_r[i] = base + token;
+      lo_r[i] = p.window > 0 ? max(0, pos_r[i] - p.window + 1) : 0;
+#pragma unroll
+      for (int t = 0; t < M::DT; ++t) o[i * M::DT + t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[i] = -INFINITY;
+      l_part[i] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < RG * M::KS; ++k)
+      asm volatile("" : "+v"(qf[k].x), "+v"(qf[k].y), "+v"(qf[k].z), "+v"(qf[k].w));
+    // what all, and what any, of the wave's rows see
+    const int pos_first = base + min(wrow, n - 1) / g, pos_last = base + min(wrow + 16 * RG - 1, n - 1) / g;
+    const int lo_last = p.window > 0 ? max(0, pos_last - p.window + 1) : 0;
+    const int lo_first = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
+    const bool rows_here = wrow < n;
+
+    for (int ch = 0; ch < count; ++ch) {
+      const int k0 = (c0 + ch) * KC;
+      const unsigned char* keys = ring[ch & 1];
+      unsigned char* vals = ring[ch & 1] + kHalf;
+      dma_stage_sync<0>();  // this chunk has landed, and every wave is done with the other buffer
+      if (ch + 1 < count) issue(c0 + ch + 1, (ch + 1) & 1);
+      if (k0 < lo_pos || k0 + KC > hi_pos) {
+        // positions that no row of the block sees may hold anything, and 0 times a NaN would be one
+        for (int y = tid; y < KC * R::kPieces; y += 64 * NW) {
+          const int key = k0 + y / R::kPieces;
+          if (key < lo_pos || key >= hi_pos) *reinterpret_cast<uint4*>(vals + y * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      if (!rows_here || k0 > pos_last || k0 + KC <= lo_first) continue;
+      f32x4 s[KT * RG];
+#pragma unroll
+      for (int j = 0; j < KT; ++j) M::template scores<RG>(keys, 16 * j, qf, s + j * RG, fr, fg);
+      const bool whole = k0 >= lo_last && k0 + KC <= pos_first + 1;
+      float mx[RG];
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        mx[i] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float y = score<T, CAP>(p, s[j * RG + i][r]);
+            if (!whole) {
+              const int key = k0 + 16 * j + 4 * fg + r;
+              y = key >= lo_r[i] && key <= pos_r[i] ? y : -INFINITY;
+            }
+            s[j * RG + i][r] = y;
+            mx[i] = fmaxf(mx[i], y);
+          }
+        grow |= mx[i] > m_run[i] + 8.f;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+          float v = fmaxf(mx[i], __shfl_xor(mx[i], 16, 64));
+          v = fmaxf(v, __shfl_xor(v, 32, 64));
+          const float m_new = v > m_run[i] + 8.f ? v : m_run[i];
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[i] - m_new);
+          l_part[i] *= alpha;
+#pragma unroll
+          for (int t = 0; t < M::DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i * M::DT + t][r] *= alpha;
+          m_run[i] = m_new;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        const float m_ref = m_run[i] == -INFINITY ? 0.f : m_run[i];
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float y = __builtin_amdgcn_exp2f(s[j * RG + i][r] - m_ref);
+            s[j * RG + i][r] = y;
+            l_part[i] += y;
+          }
+      }
+      M::template values<KT, RG>(vals, s, o, lane);
+    }
+    const bool all = count == x.chunks;
+    const int64_t slot = ((int64_t)2 * w + (first_item ? 0 : 1)) * BQ;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+      float l = l_part[i] + __shfl_xor(l_part[i], 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      const int r = wrow + 16 * i + fr, token = r / g;
+      if (r >= n) continue;
+      if (all) {
+        T* orow = (T*)p.out + (int64_t)(q.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(orow + d, y * inv); });
+      } else {
+        const int64_t at_row = slot + r - row0;
+        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(p.part_o + at_row * D + d, y); });
+        if (fg == 0) p.part_ml[at_row] = make_float2(m_run[i], l);
+      }
+    }
+    first_item = false;
+    at += count;
+    if (at < stop) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // both buffers are free
+  }
+}
+
+// Joins the parts of blocks that a run's border cut, and writes zeros for blocks that see nothing. One
+// workgroup per 16 rows of a (block, kv head).
+template <typename T, int D, int BQ>
+__global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const int* total) {
+  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+  const int tid = threadIdx.x, g = p.b.Hq / p.b.Hkv;
+  const int line = total[0], tiles = total[1 + p.b.n_seqs];
+  const int t = blockIdx.x, h = blockIdx.y;
+  if (t >= tiles) return;
+  const PagedTile x = p.tiles[t];
+  const int per = tile_run(p, line), a = h * line + x.at;
+  const int wa = x.chunks > 0 ? a / per : 0, parts = x.chunks > 0 ? (a + x.chunks - 1) / per - wa + 1 : 0;
+  if (parts == 1) return;
+  const PagedSeq q = paged_seq(p.b, x.seq, false);
+  const int n = min(q.n, p.max_q) * g, last = min(x.row + (int)(blockIdx.z + 1) * 16, n);
+  const int lane = tid % kLanes;
+  for (int r = x.row + blockIdx.z * 16 + tid / kLanes; r < last; r += kRows) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f, m = -INFINITY;
+    auto slot = [&](int k) -> int64_t {
+      return ((int64_t)2 * (wa + k) + (k > 0 || a == wa * per ? 0 : 1)) * BQ + r - x.row;
+    };
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[slot(k)].x);
+    if (m == -INFINITY) m = 0.f;
+    for (int k = 0; k < parts; ++k) {
+      const int64_t s = slot(k);
+      const float2 ml = p.part_ml[s];
+      const float e = __builtin_amdgcn_exp2f(ml.x - m);
+      l += e * ml.y;
+      o += e * *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * lane);
+    }
+    const int token = r / g;
+    T* orow = (T*)p.out + (int64_t)(q.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
+    store_run(orow + 4 * lane, o * (l > 0.f ? 1.f / l : 0.f));
+  }
+}
 
 // ---------------------------------------------------------------------------------------
 // launches
@@ -651,6 +913,49 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   return TL_OK;
 }
 
+// Blocks of the tile kernel: 128 rows, two 16-row groups a wave while their outputs fit the registers of
+// two waves a SIMD; fp32 64 rows. As many workgroups as LDS and registers hold at a time.
+template <typename T, int D>
+struct TileShape {
+  static constexpr bool kBf = sizeof(T) == 2;
+  static constexpr int NW = kBf && D == 256 ? 8 : 4, RG = kBf && D < 256 ? 2 : 1, KC = kBf ? 64 : 32;
+  static constexpr int BQ = 16 * NW * RG;
+  static constexpr int kLds = 4 * KC * D * (int)sizeof(T);
+  static constexpr int kPerCu = std::min(160 * 1024 / kLds, kBf ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : 2);
+};
+
+template <typename T, int D>
+static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
+  using S = TileShape<T, D>;
+  const int64_t g = p.b.Hq / p.b.Hkv;
+  const int64_t most = std::min<int64_t>(p.b.n_seqs, p.b.n_rows) + (int64_t)p.b.n_rows * g / S::BQ;
+  const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
+  TL_REQUIRE(line * p.b.Hkv < (1LL << 30), "batch too large: row blocks x kv heads x table positions");
+  TL_REQUIRE(p.b.Hkv <= 65535, "more than 65535 kv heads");
+  const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+  p.workers = (int)std::max<int64_t>(8, (int64_t)S::kPerCu * cus / 8 * 8);
+  p.most_tiles = (int)most;
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t obytes = up((size_t)p.workers * 2 * S::BQ * D * sizeof(float));
+  const size_t mbytes = up((size_t)p.workers * 2 * S::BQ * sizeof(float2));
+  const size_t tbytes = up((size_t)most * sizeof(PagedTile));
+  void* ws;
+  const int rc = workspace(ctx, obytes + mbytes + tbytes + ((size_t)p.b.n_seqs + 2) * sizeof(int), &ws);
+  if (rc) return rc;
+  p.part_o = (float*)ws;
+  p.part_ml = (float2*)((char*)ws + obytes);
+  p.tiles = (PagedTile*)((char*)ws + obytes + mbytes);
+  int* total = (int*)((char*)ws + obytes + mbytes + tbytes);
+  paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
+  if (p.cap > 0.f)
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+  else
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+  paged_tile_join_kernel<T, D, S::BQ>
+      <<<dim3((unsigned)most, (unsigned)p.b.Hkv, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
+  return TL_OK;
+}
+
 template <typename T, int D>
 static int launch_attention(tl_ctx* ctx, PagedAttn p) {
   const int64_t g = p.b.Hq / p.b.Hkv;
@@ -658,8 +963,7 @@ static int launch_attention(tl_ctx* ctx, PagedAttn p) {
     p.skip = 0;
     return launch_step<T, D>(ctx, p);
   }
-  paged_attention_simple_kernel<T, D><<<(unsigned)(p.b.n_rows * p.b.Hq), 64, 0, ctx->stream>>>(p);
-  return TL_OK;
+  return launch_tiles<T, D>(ctx, p);
 }
 
 }  // namespace tl
