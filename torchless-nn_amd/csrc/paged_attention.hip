@@ -27,6 +27,10 @@ struct PagedAttn {
   float* part_o;
   float2* part_ml;
   int workers;
+  // the shared prefix: its chunks cut into `splits` for each of row_blocks blocks of the batch's rows
+  float* pre_o;
+  float2* pre_ml;
+  int splits, row_blocks;
   // the tile kernel's plan: row blocks of the batch, in order; per kv head they are one line of chunks
   PagedTile* tiles;
   int most_tiles;
@@ -483,13 +487,15 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
       l += __shfl_xor(l, 32, 64);
       const bool all = last && c_first == cp.q.lo / KC;
       if (fr < cp.q.n * g) {
-        if (all) {
+        if (all && p.skip == 0) {
           T* orow = (T*)p.out + (int64_t)(cp.q.row0 + token) * p.ld_out + head * D;
           const float inv = l > 0.f ? 1.f / l : 0.f;
           M::each_run(o, fg, [&](int d, f32x4 x) { store_run(orow + d, x * inv); });
         } else {
-          // a run has at most two items that it does not hold whole: the one it begins in, and its last
-          const int64_t slot = (int64_t)(2 * w + (first_item ? 0 : 1)) * (p.max_q * g) + fr;
+          // a run has at most two items that it does not hold whole: the one it begins in, and its last;
+          // whole ones that the prefix is still to be joined to come after those of all runs
+          const int64_t slot = all ? (int64_t)2 * p.workers * (p.max_q * g) + (int64_t)(cp.q.row0 + token) * p.b.Hq + head
+                                   : (int64_t)(2 * w + (first_item ? 0 : 1)) * (p.max_q * g) + fr;
           float* orow = p.part_o + slot * D;
           M::each_run(o, fg, [&](int d, f32x4 x) { store_run(orow + d, x); });
           if (fg == 0) p.part_ml[slot] = make_float2(m_run, l);
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
 // largest m_i. Also what the step kernel has no chunk for: zeros for rows that see nothing, and the
 // report of bounds that are out of range. Every workgroup finds its parts from the lengths, as the
 // step kernel found its runs; the parts are taken in their order, so results repeat bit for bit.
-template <typename T, int D, int KC>
+template <typename T, int D, int KC, int PBQ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads of a part, parts at a time
   __shared__ int sums[4][2];
@@ -543,20 +549,32 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   __syncthreads();
   all = (sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0]) * p.b.Hkv;
   before = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
-  if (chunks == 0) {
+  if (chunks == 0 && p.skip == 0) {
     if (tid < kLanes) store_run(orow + 4 * tid, f32x4{0.f, 0.f, 0.f, 0.f});
     return;
   }
-  const int per = (int)(((uint32_t)all + p.workers - 1) / (uint32_t)p.workers);
-  const int a = before * p.b.Hkv + (head / g) * chunks;
-  const int wa = a / per, parts = (a + chunks - 1) / per - wa + 1;
-  if (parts == 1) return;  // finished by the step kernel
-  const int rows = p.max_q * g, row = i * g + head % g;
+  int own = 0, wa = 0;  // parts of the row's own chunks
+  bool at_start = false;
+  if (chunks > 0) {
+    const int per = (int)(((uint32_t)all + p.workers - 1) / (uint32_t)p.workers);
+    const int a = before * p.b.Hkv + (head / g) * chunks;
+    wa = a / per;
+    own = (a + chunks - 1) / per - wa + 1;
+    at_start = a == wa * per;
+  }
+  if (own == 1 && p.skip == 0) return;  // finished by the step kernel
+  const int rows = p.max_q * g, row = i * g + head % g, parts = own + (p.skip > 0 ? p.splits : 0);
+  // part k: the row's own chunks', then the prefix's
   auto slot = [&](int k) -> int64_t {
-    return (int64_t)(2 * (wa + k) + (k > 0 || a == wa * per ? 0 : 1)) * rows + row;
+    if (k >= own) {
+      const int r = t * g + head % g;
+      return ((int64_t)((head / g) * p.splits + k - own) * p.row_blocks + r / PBQ) * PBQ + r % PBQ;
+    }
+    if (own == 1) return (int64_t)2 * p.workers * rows + (int64_t)t * p.b.Hq + head;
+    return (int64_t)(2 * (wa + k) + (k > 0 || at_start ? 0 : 1)) * rows + row;
   };
   float m = -INFINITY;
-  for (int k = lane; k < parts; k += 64) m = fmaxf(m, p.part_ml[slot(k)].x);
+  for (int k = lane; k < parts; k += 64) m = fmaxf(m, (k < own ? p.part_ml : p.pre_ml)[slot(k)].x);
   m = wave_max(m);
   if (m == -INFINITY) m = 0.f;
   const int grp = tid / kLanes, at = tid % kLanes;
@@ -564,10 +582,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   float l = 0.f;
   for (int k = grp; k < parts; k += kGroups) {
     const int64_t s = slot(k);
-    const float2 ml = p.part_ml[s];
+    const float2 ml = (k < own ? p.part_ml : p.pre_ml)[s];
     const float e = __builtin_amdgcn_exp2f(ml.x - m);
     l += e * ml.y;
-    o += e * *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * at);
+    o += e * *reinterpret_cast<const f32x4*>((k < own ? p.part_o : p.pre_o) + s * D + 4 * at);
   }
   acc[grp][at] = o;
   if (at == 0) lsum[grp] = l;
@@ -671,7 +689,10 @@ __device__ __forceinline__ int tile_run(const PagedAttn& p, int line) {
   return (int)(((uint32_t)line * p.b.Hkv + p.workers - 1) / (uint32_t)p.workers);
 }
 
-template <typename T, int D, int NW, int RG, int KC, bool CAP>
+// The same for a shared prefix (PREFIX): all rows of the batch as one sequence that sees positions 0 ..
+// skip - 1 whole, each workgroup one part of them for one block of rows; always parts, which the step
+// kernel's join takes in.
+template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PREFIX>
 __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const int* total) {
   using R = Rows<T, D>;
   using M = Tile16<T, D>;
@@ -680,29 +701,56 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int g = p.b.Hq / p.b.Hkv;
   // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
-  const int w = (int)(blockIdx.x % 8) * (p.workers / 8) + (int)(blockIdx.x / 8);
-  const int line = total[0], tiles = total[1 + p.b.n_seqs];
-  const int per = tile_run(p, line);
-  int at = w * per;
-  const int stop = min(line * p.b.Hkv, at + per);
+  const int w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
+  int line = 1, tiles = 0, at = w, stop = min(w + 1, p.b.Hkv * p.splits * p.row_blocks);
+  if constexpr (!PREFIX) {
+    line = total[0];
+    tiles = total[1 + p.b.n_seqs];
+    const int per = tile_run(p, line);
+    at = w * per;
+    stop = min(line * p.b.Hkv, at + per);
+  }
   const uint32_t ring0 = lds_offset(ring);
   bool first_item = true;
   while (at < stop) {
-    const int h = at / line, off = at - h * line;
-    int lo = 0, hi = tiles;  // the last tile that starts at or before off and has chunks
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.tiles[mid].at <= off) lo = mid;
-      else hi = mid;
+    int h, c0, count, chunks, seq_row, base, n, row0, hi_pos, lo_pos;
+    const int32_t* pages = p.b.table;
+    if constexpr (PREFIX) {
+      h = at / (p.splits * p.row_blocks);
+      const int split = at / p.row_blocks % p.splits, all = (p.skip + KC - 1) / KC;
+      c0 = (int)((int64_t)split * all / p.splits);
+      count = (int)((int64_t)(split + 1) * all / p.splits) - c0;
+      chunks = seq_row = 0;
+      row0 = at % p.row_blocks * BQ;
+      n = p.b.n_rows * g;
+      base = p.skip - 1;
+      hi_pos = p.skip;
+      lo_pos = 0;
+    } else {
+      h = at / line;
+      const int off = at - h * line;
+      int lo = 0, hi = tiles;  // the last tile that starts at or before off: it has chunks
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.tiles[mid].at <= off) lo = mid;
+        else hi = mid;
+      }
+      const PagedTile x = p.tiles[lo];
+      c0 = uniform(x.chunk0 + off - x.at);
+      count = uniform(min(x.at + x.chunks - off, stop - at));
+      chunks = uniform(x.chunks);
+      const int seq = uniform(x.seq);
+      const PagedSeq q = paged_seq(p.b, seq, false);
+      seq_row = uniform(q.row0);
+      n = uniform(min(q.n, p.max_q) * g);
+      base = uniform(q.len - q.n);
+      row0 = uniform(x.row);
+      hi_pos = base + (min(row0 + BQ, n) - 1) / g + 1;
+      lo_pos = max(0, p.window > 0 ? base + row0 / g - p.window + 1 : 0);
+      pages += (int64_t)seq * p.b.ld_table;
     }
-    const PagedTile x = p.tiles[lo];
-    const int c0 = uniform(x.chunk0 + off - x.at), count = uniform(min(x.at + x.chunks - off, stop - at));
-    const int seq = uniform(x.seq);
-    const PagedSeq q = paged_seq(p.b, seq, false);
-    const int n = uniform(min(q.n, p.max_q) * g), base = uniform(q.len - q.n), row0 = uniform(x.row);
-    const int hi_pos = base + (min(row0 + BQ, n) - 1) / g + 1;
-    const int lo_pos = max(0, p.window > 0 ? base + row0 / g - p.window + 1 : 0);
-    const int32_t* pages = p.b.table + (int64_t)seq * p.b.ld_table;
+    // the position of the block's row r
+    auto position = [&](int r) { return PREFIX ? base : base + r / g; };
 
     auto issue = [&](int c, int stage) {
 #pragma unroll
@@ -732,11 +780,11 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
       const int r = min(wrow + 16 * i + fr, n - 1), token = r / g;
-      const T* qr = (const T*)p.q + (int64_t)(q.row0 + token) * p.ld_q + (h * g + r - token * g) * D;
+      const T* qr = (const T*)p.q + (int64_t)(seq_row + token) * p.ld_q + (h * g + r - token * g) * D;
 #pragma unroll
       for (int ks = 0; ks < M::KS; ++ks)
         qf[i * M::KS + ks] = *reinterpret_cast<const uint4*>(qr + (4 * ks + fg) * R::kVec);
-      pos_r[i] = base + token;
+      pos_r[i] = position(r);
       lo_r[i] = p.window > 0 ? max(0, pos_r[i] - p.window + 1) : 0;
 #pragma unroll
       for (int t = 0; t < M::DT; ++t) o[i * M::DT + t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -747,7 +795,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     for (int k = 0; k < RG * M::KS; ++k)
       asm volatile("" : "+v"(qf[k].x), "+v"(qf[k].y), "+v"(qf[k].z), "+v"(qf[k].w));
     // what all, and what any, of the wave's rows see
-    const int pos_first = base + min(wrow, n - 1) / g, pos_last = base + min(wrow + 16 * RG - 1, n - 1) / g;
+    const int pos_first = position(min(wrow, n - 1)), pos_last = position(min(wrow + 16 * RG - 1, n - 1));
     const int lo_last = p.window > 0 ? max(0, pos_last - p.window + 1) : 0;
     const int lo_first = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
     const bool rows_here = wrow < n;
@@ -819,22 +867,24 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       }
       M::template values<KT, RG>(vals, s, o, lane);
     }
-    const bool all = count == x.chunks;
-    const int64_t slot = ((int64_t)2 * w + (first_item ? 0 : 1)) * BQ;
+    const bool all = count == chunks;
+    const int64_t slot = (PREFIX ? (int64_t)w : (int64_t)2 * w + (first_item ? 0 : 1)) * BQ;
+    float* part_o = PREFIX ? p.pre_o : p.part_o;
+    float2* part_ml = PREFIX ? p.pre_ml : p.part_ml;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
       float l = l_part[i] + __shfl_xor(l_part[i], 16, 64);
       l += __shfl_xor(l, 32, 64);
       const int r = wrow + 16 * i + fr, token = r / g;
       if (r >= n) continue;
-      if (all) {
-        T* orow = (T*)p.out + (int64_t)(q.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
+      if (!PREFIX && all) {
+        T* orow = (T*)p.out + (int64_t)(seq_row + token) * p.ld_out + (h * g + r - token * g) * D;
         const float inv = l > 0.f ? 1.f / l : 0.f;
         M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(orow + d, y * inv); });
       } else {
         const int64_t at_row = slot + r - row0;
-        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(p.part_o + at_row * D + d, y); });
-        if (fg == 0) p.part_ml[at_row] = make_float2(m_run[i], l);
+        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(part_o + at_row * D + d, y); });
+        if (fg == 0) part_ml[at_row] = make_float2(m_run[i], l);
       }
     }
     first_item = false;
@@ -894,25 +944,6 @@ struct StepShape {
   static constexpr int kPerCu = (160 * 1024) / kLds < 8 ? (160 * 1024) / kLds : 8;
 };
 
-template <typename T, int D>
-static int launch_step(tl_ctx* ctx, PagedAttn p) {
-  using S = StepShape<T, D>;
-  const int64_t rows = (int64_t)p.max_q * (p.b.Hq / p.b.Hkv);
-  const int64_t most = (int64_t)p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
-  TL_REQUIRE(most < (1LL << 30), "batch too large: sequences x kv heads x table positions");
-  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)S::kPerCu * (ctx->num_cus > 0 ? ctx->num_cus : 256)));
-  const size_t obytes = (size_t)p.workers * 2 * rows * D * sizeof(float);
-  void* ws;
-  const int rc = workspace(ctx, obytes + (size_t)p.workers * 2 * rows * sizeof(float2), &ws);
-  if (rc) return rc;
-  p.part_o = (float*)ws;
-  p.part_ml = (float2*)((char*)ws + obytes);
-  if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
-  else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
-  paged_join_kernel<T, D, S::KC><<<(unsigned)(p.b.n_rows * p.b.Hq), 256, 0, ctx->stream>>>(p);
-  return TL_OK;
-}
-
 // Blocks of the tile kernel: 128 rows, two 16-row groups a wave while their outputs fit the registers of
 // two waves a SIMD; fp32 64 rows. As many workgroups as LDS and registers hold at a time.
 template <typename T, int D>
@@ -923,6 +954,50 @@ struct TileShape {
   static constexpr int kLds = 4 * KC * D * (int)sizeof(T);
   static constexpr int kPerCu = std::min(160 * 1024 / kLds, kBf ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : 2);
 };
+
+static size_t aligned256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+template <typename T, int D>
+static int launch_step(tl_ctx* ctx, PagedAttn p) {
+  using S = StepShape<T, D>;
+  using P = TileShape<T, D>;
+  const int64_t g = p.b.Hq / p.b.Hkv, rows = p.max_q * g, heads = (int64_t)p.b.n_rows * p.b.Hq;
+  const int64_t most = (int64_t)p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
+  TL_REQUIRE(most < (1LL << 30), "batch too large: sequences x kv heads x table positions");
+  const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)S::kPerCu * cus));
+  p.skip = p.shared;
+  int64_t blocks = 0;  // of the prefix kernel
+  p.row_blocks = p.splits = 0;
+  if (p.skip > 0) {
+    p.row_blocks = (int)((p.b.n_rows * g + P::BQ - 1) / P::BQ);
+    const int64_t lines = (int64_t)p.row_blocks * p.b.Hkv, chunks = (p.skip + P::KC - 1) / P::KC;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, (int64_t)P::kPerCu * cus / lines));
+    blocks = lines * p.splits;
+    TL_REQUIRE(blocks < (1LL << 30), "batch too large: row blocks x kv heads x prefix");
+  }
+  const int64_t slots = 2LL * p.workers * rows + (p.skip > 0 ? heads : 0), pre = blocks * P::BQ;
+  const size_t obytes = aligned256((size_t)slots * D * sizeof(float)), mbytes = aligned256((size_t)slots * sizeof(float2));
+  const size_t pbytes = aligned256((size_t)pre * D * sizeof(float));
+  void* ws;
+  const int rc = workspace(ctx, obytes + mbytes + pbytes + (size_t)pre * sizeof(float2), &ws);
+  if (rc) return rc;
+  p.part_o = (float*)ws;
+  p.part_ml = (float2*)((char*)ws + obytes);
+  p.pre_o = (float*)((char*)ws + obytes + mbytes);
+  p.pre_ml = (float2*)((char*)ws + obytes + mbytes + pbytes);
+  if (p.skip > 0) {
+    const unsigned grid = (unsigned)((blocks + 7) / 8 * 8);
+    if (p.cap > 0.f)
+      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, true, true><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+    else
+      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, false, true><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+  }
+  if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
+  else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
+  paged_join_kernel<T, D, S::KC, P::BQ><<<(unsigned)heads, 256, 0, ctx->stream>>>(p);
+  return TL_OK;
+}
 
 template <typename T, int D>
 static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
@@ -935,10 +1010,9 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
   p.workers = (int)std::max<int64_t>(8, (int64_t)S::kPerCu * cus / 8 * 8);
   p.most_tiles = (int)most;
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  const size_t obytes = up((size_t)p.workers * 2 * S::BQ * D * sizeof(float));
-  const size_t mbytes = up((size_t)p.workers * 2 * S::BQ * sizeof(float2));
-  const size_t tbytes = up((size_t)most * sizeof(PagedTile));
+  const size_t obytes = aligned256((size_t)p.workers * 2 * S::BQ * D * sizeof(float));
+  const size_t mbytes = aligned256((size_t)p.workers * 2 * S::BQ * sizeof(float2));
+  const size_t tbytes = aligned256((size_t)most * sizeof(PagedTile));
   void* ws;
   const int rc = workspace(ctx, obytes + mbytes + tbytes + ((size_t)p.b.n_seqs + 2) * sizeof(int), &ws);
   if (rc) return rc;
@@ -948,9 +1022,9 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   int* total = (int*)((char*)ws + obytes + mbytes + tbytes);
   paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
   if (p.cap > 0.f)
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   else
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   paged_tile_join_kernel<T, D, S::BQ>
       <<<dim3((unsigned)most, (unsigned)p.b.Hkv, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
   return TL_OK;
@@ -959,10 +1033,8 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
 template <typename T, int D>
 static int launch_attention(tl_ctx* ctx, PagedAttn p) {
   const int64_t g = p.b.Hq / p.b.Hkv;
-  if (p.max_q * g <= 16) {
-    p.skip = 0;
-    return launch_step<T, D>(ctx, p);
-  }
+  if (p.max_q * g <= 16) return launch_step<T, D>(ctx, p);
+  p.skip = 0;
   return launch_tiles<T, D>(ctx, p);
 }
 
