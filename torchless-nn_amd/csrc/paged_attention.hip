@@ -123,28 +123,45 @@ struct Tile16 {
   static constexpr int DT = D / 16;                  // output tiles
   static constexpr int E = DT < 4 ? DT : 4;          // fp32: consecutive outputs that one read feeds
 
-  // Scores of 16 keys from row `row0` of a chunk against RG groups of 16 queries (q[group][KS])
-  template <int RG>
-  __device__ __forceinline__ static void scores(const unsigned char* keys, int row0, const uint4* q, f32x4* s, int fr,
-                                                int fg) {
-    const int row = row0 + fr, sw = R::key_swizzle(row);
+  // Scores of KT tiles of 16 keys of a chunk against RG groups of 16 queries: q[group][KS] to
+  // s[tile][group]. The reads of a few fragments run ahead of the products that take them.
+  template <int KT, int RG>
+  __device__ __forceinline__ static void scores(const unsigned char* keys, const uint4* q, f32x4* s, int fr, int fg) {
+    const int sw = R::key_swizzle(fr);
 #pragma unroll
-    for (int i = 0; i < RG; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < KT * RG; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + row * R::kBytes + (((4 * ks + fg) ^ sw) << 4));
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < RG; ++i) {
-        if constexpr (kBf) {
-          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
-                                                         __builtin_bit_cast(bf16x8, q[i * KS + ks]), s[i], 0, 0, 0);
-        } else {
-          const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[i * KS + ks]);
+      for (int j = 0; j < KT; ++j) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + (16 * j + fr) * R::kBytes + (((4 * ks + fg) ^ sw) << 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], s[i], 0, 0, 0);
+        for (int i = 0; i < RG; ++i) {
+          f32x4& x = s[j * RG + i];
+          if constexpr (kBf) {
+            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
+                                                        __builtin_bit_cast(bf16x8, q[i * KS + ks]), x, 0, 0, 0);
+          } else {
+            const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[i * KS + ks]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], x, 0, 0, 0);
+          }
         }
       }
+    pipeline<KT * KS, KT * KS < 6 ? KT * KS : 6, kBf ? RG : 4 * RG, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // The order of a region of `reads` x PER LDS reads that feed MFMAS products each: AHEAD of them first,
+  // then one (PER reads) for every MFMAS products.
+  template <int READS, int AHEAD, int MFMAS, int PER>
+  __device__ __forceinline__ static void pipeline() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * PER, 0);
+#pragma unroll
+    for (int i = 0; i < READS - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD * MFMAS, 0);
   }
   // The bf16 operand V^T[16 t .. +15][32 keys] of keys 4 fg .. +3 and 16 + 4 fg .. +3 of `half`
   __device__ __forceinline__ static bf16x8 value_frag(const unsigned char* values, int half, int t, int lane) {
@@ -178,6 +195,7 @@ struct Tile16 {
             o[i * DT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[i], o[i * DT + t], 0, 0, 0);
         }
       }
+      pipeline<KT / 2 * DT, KT / 2 * DT < 5 ? KT / 2 * DT : 5, RG, 2>();
     } else {
       const int fr = lane & 15, fg = lane >> 4;
 #pragma unroll
@@ -198,7 +216,9 @@ struct Tile16 {
                     __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], s[j * RG + i][r], o[i * DT + t * E + e], 0, 0, 0);
           }
         }
+      pipeline<KT * 4 * (DT / E), 4, E * RG, 1>();
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
   // Calls f(d, x) for runs of 4 consecutive outputs x of the lane's query row, at d .. d + 3 (fp32 at
   // D = 32: 2 runs of 4 all the same).
@@ -234,6 +254,34 @@ __device__ __forceinline__ float score(const PagedAttn& p, float s) {
   if constexpr (sizeof(T) == 4) return p.cap * tanhf(s * p.cap_in * 0.34657359027997264f);
   const float e = __builtin_amdgcn_exp2f(s * p.cap_in);
   return __builtin_fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(1.f + e), p.cap);
+}
+
+// The scores of KT x 16 keys from k0 on of one group (every RG-th of s) in log2 units, those of positions
+// outside lo .. hi at -inf unless all are inside (`whole`, uniform); returns the lane's largest.
+template <typename T, bool CAP, int KT, int RG>
+__device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool whole, int first, int lo, int hi) {
+  float mx = -INFINITY;
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[j * RG][r] = score<T, CAP>(p, s[j * RG][r]);
+        mx = fmaxf(mx, s[j * RG][r]);
+      }
+  } else {
+    // the lane's key 16 j + r of the chunk is position first + 16 j + r
+    const int a = lo - first, n = hi - lo;
+#pragma unroll
+    for (int j = 0; j < KT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float y = score<T, CAP>(p, s[j * RG][r]);
+        s[j * RG][r] = hi >= lo && (uint32_t)(16 * j + r - a) <= (uint32_t)n ? y : -INFINITY;
+        mx = fmaxf(mx, s[j * RG][r]);
+      }
+  }
+  return mx;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -354,19 +402,25 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
   StepCursor<KC> cp = ld;
 
   const uint32_t ring0 = lds_offset(ring);
+  const int count = end - begin;
+  int queued = 0;
+  // the pages of the chunk to be queued next, looked up a chunk ahead; a block of 16 positions without a
+  // visible one is read from page 0: its scores are masked, its values zeroed
+  int id[KT];
+  bool bad = false;
+  auto look_up = [&]() {
+    ConstInts row = const_ints(p.b.table) + (int64_t)ld.s * p.b.ld_table;
+#pragma unroll
+    for (int j = 0; j < KT; ++j) id[j] = uniform(row[min((ld.c * KC + 16 * j) >> p.b.page_shift, p.b.cols - 1)]);
+  };
   auto issue = [&](int stage) {
     const int k0 = ld.c * KC;
-    ConstInts row = const_ints(p.b.table) + (int64_t)ld.s * p.b.ld_table;
-    int id[KT];
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
-      // a block without a visible position is read from page 0: its scores are masked, its values zeroed
       const int pos = k0 + 16 * j;
-      const bool use = pos < ld.q.hi && pos + 16 > ld.q.lo;
-      const int x = uniform(row[min(pos >> p.b.page_shift, p.b.cols - 1)]);
-      const bool ok = (uint32_t)x < (uint32_t)p.b.n_pages;
-      if (use && !ok && lane == 0) latch(p.b.status, kBadPage);
-      id[j] = use && ok ? x : 0;
+      const bool use = pos < ld.q.hi && pos + 16 > ld.q.lo, ok = (uint32_t)id[j] < (uint32_t)p.b.n_pages;
+      bad |= use && !ok;
+      id[j] = use && ok ? id[j] : 0;
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
@@ -380,17 +434,15 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
         else load_block16<T, D, true>(uniform(src), uniform(lds), lane);
       }
     }
+    ld.next(p);
+    ++queued;
+    if (queued < count) look_up();
   };
 
-  const int count = end - begin;
-  int queued = 0;
+  look_up();
 #pragma unroll
   for (int st = 0; st < ST; ++st)
-    if (queued < count) {
-      issue(st);
-      ld.next(p);
-      ++queued;
-    }
+    if (queued < count) issue(st);
 
   uint4 qf[M::KS];
   f32x4 o[M::DT];
@@ -422,25 +474,13 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
     unsigned char* vals = ring + stage * kStage + kHalf;
     wait_loads<kLoads, (2 * ST - 1) * kLoads>(ahead + kLoads);
     f32x4 s[KT];
-#pragma unroll
-    for (int j = 0; j < KT; ++j) M::template scores<1>(keys, 16 * j, qf, s + j, fr, fg);
+    M::template scores<KT, 1>(keys, qf, s, fr, fg);
 
     const int k0 = cp.c * KC;
     const int pos = cp.q.base + token;
     const int lo = max(p.skip, p.window > 0 ? pos - p.window + 1 : 0);
     const bool whole = k0 >= max(p.skip, p.window > 0 ? cp.q.hi - p.window : 0) && k0 + KC <= cp.q.base + 1;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < KT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[j][r] = score<T, CAP>(p, s[j][r]);
-        if (!whole) {
-          const int key = k0 + 16 * j + 4 * fg + r;
-          s[j][r] = key >= lo && key <= pos ? s[j][r] : -INFINITY;
-        }
-        mx = fmaxf(mx, s[j][r]);
-      }
+    float mx = mask_scores<T, CAP, KT, 1>(p, s, whole, k0 + 4 * fg, lo, pos);
     // the reference maximum moves only when a score passes it by more than 2^8, and only then the
     // row's four lanes are asked (unnormalised probabilities stay below 2^8)
     if (__any(mx > m_run + 8.f)) {
@@ -474,11 +514,7 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
     M::template values<KT, 1>(vals, s, o, lane);
     // the stage is free once its reads have returned
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (queued < count) {
-      issue(stage);
-      ld.next(p);
-      ++queued;
-    }
+    if (queued < count) issue(stage);
     stage = stage + 1 == ST ? 0 : stage + 1;
 
     const bool last = cp.c + 1 == (cp.q.hi + KC - 1) / KC;
@@ -506,6 +542,7 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
     }
     cp.next(p);
   }
+  if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
 
 // Joins the parts of one (row, query head): out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m the
@@ -711,7 +748,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     stop = min(line * p.b.Hkv, at + per);
   }
   const uint32_t ring0 = lds_offset(ring);
-  bool first_item = true;
+  bool first_item = true, bad = false;
   while (at < stop) {
     int h, c0, count, chunks, seq_row, base, n, row0, hi_pos, lo_pos;
     const int32_t* pages = p.b.table;
@@ -752,24 +789,35 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     // the position of the block's row r
     auto position = [&](int r) { return PREFIX ? base : base + r / g; };
 
+    // the wave's blocks of 16 positions in every chunk (keys' blocks, then values'), their pages looked up a
+    // chunk ahead; one that no row of the block of rows sees is read from page 0 (masked, and zeroed)
+    constexpr int kMine = (2 * KT + NW - 1) / NW;
+    int id[kMine];
+    auto look_up = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int pos = c * KC + 16 * ((i * NW + wave) % KT);
+        id[i] = uniform(const_ints(pages)[min(pos >> p.b.page_shift, p.b.cols - 1)]);
+      }
+    };
     auto issue = [&](int c, int stage) {
 #pragma unroll
-      for (int b = 0; b < 2 * KT; b += NW) {
-        const int blk = b + wave;  // keys' blocks, then values'
+      for (int i = 0; i < kMine; ++i) {
+        const int blk = i * NW + wave;
         if (2 * KT % NW != 0 && blk >= 2 * KT) break;
         const int j = blk % KT, pos = c * KC + 16 * j;
-        const bool use = pos < hi_pos && pos + 16 > lo_pos;
-        const int id = const_ints(pages)[min(pos >> p.b.page_shift, p.b.cols - 1)];
-        const bool ok = (uint32_t)id < (uint32_t)p.b.n_pages;
-        if (use && !ok && lane == 0) latch(p.b.status, kBadPage);
+        const bool use = pos < hi_pos && pos + 16 > lo_pos, ok = (uint32_t)id[i] < (uint32_t)p.b.n_pages;
+        bad |= use && !ok;
         const int slot = pos & ((1 << p.b.page_shift) - 1);
-        const int64_t from = ((((int64_t)(use && ok ? id : 0) * p.b.Hkv + h) << p.b.page_shift) + slot) * R::kBytes;
+        const int64_t from = ((((int64_t)(use && ok ? id[i] : 0) * p.b.Hkv + h) << p.b.page_shift) + slot) * R::kBytes;
         const int lds = (int)ring0 + stage * 2 * kHalf + (blk / KT) * kHalf + j * 16 * R::kBytes;
         if (blk < KT) load_block16<T, D, true>(uniform((const unsigned char*)p.k + from), uniform(lds), lane);
         else load_block16<T, D, false>(uniform((const unsigned char*)p.v + from), uniform(lds), lane);
       }
     };
+    look_up(c0);
     issue(c0, 0);
+    if (count > 1) look_up(c0 + 1);
 
     // this wave's rows
     uint4 qf[RG * M::KS];
@@ -806,6 +854,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       unsigned char* vals = ring[ch & 1] + kHalf;
       dma_stage_sync<0>();  // this chunk has landed, and every wave is done with the other buffer
       if (ch + 1 < count) issue(c0 + ch + 1, (ch + 1) & 1);
+      if (ch + 2 < count) look_up(c0 + ch + 2);
       if (k0 < lo_pos || k0 + KC > hi_pos) {
         // positions that no row of the block sees may hold anything, and 0 times a NaN would be one
         for (int y = tid; y < KC * R::kPieces; y += 64 * NW) {
@@ -816,26 +865,13 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       }
       if (!rows_here || k0 > pos_last || k0 + KC <= lo_first) continue;
       f32x4 s[KT * RG];
-#pragma unroll
-      for (int j = 0; j < KT; ++j) M::template scores<RG>(keys, 16 * j, qf, s + j * RG, fr, fg);
+      M::template scores<KT, RG>(keys, qf, s, fr, fg);
       const bool whole = k0 >= lo_last && k0 + KC <= pos_first + 1;
       float mx[RG];
       bool grow = false;
 #pragma unroll
       for (int i = 0; i < RG; ++i) {
-        mx[i] = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < KT; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float y = score<T, CAP>(p, s[j * RG + i][r]);
-            if (!whole) {
-              const int key = k0 + 16 * j + 4 * fg + r;
-              y = key >= lo_r[i] && key <= pos_r[i] ? y : -INFINITY;
-            }
-            s[j * RG + i][r] = y;
-            mx[i] = fmaxf(mx[i], y);
-          }
+        mx[i] = mask_scores<T, CAP, KT, RG>(p, s + i, whole, k0 + 4 * fg, lo_r[i], pos_r[i]);
         grow |= mx[i] > m_run[i] + 8.f;
       }
       if (__any(grow)) {
@@ -891,6 +927,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     at += count;
     if (at < stop) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // both buffers are free
   }
+  if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
 
 // Joins the parts of blocks that a run's border cut, and writes zeros for blocks that see nothing. One
