@@ -6,10 +6,11 @@
 
 namespace tl {
 
-// A block of a sequence's rows (row r: token r / g, query head r % g of the kv head's) and the chunks
-// that they see: chunk0 .. chunk0 + chunks - 1, which lie at `at` on the line.
-struct PagedTile {
-  int seq, row, chunk0, chunks, at;
+// A block of a sequence's rows (row r: token r / g, query head r % g of the kv head's), from `row` on, and
+// the chunks that they see: chunk0 .. chunk0 + chunks - 1, which lie from `at` on on the line. The sequence's
+// tokens begin at row row0 of the batch and at position base; it has n rows.
+struct __attribute__((aligned(32))) PagedTile {
+  int seq, row, chunk0, chunks, at, row0, base, n;
 };
 
 struct PagedAttn {
@@ -356,9 +357,10 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
 
   // this wave's run [begin, end) of the line of chunks, and where it begins
   int total = 0, mine = 0;
+  PagedSeq raw = {};
   for (int s = lane; s < p.b.n_seqs; s += 64) {
-    const PagedSeq q = paged_seq(p.b, s, false);
-    mine = step_chunks<KC>(step_seq(p, q.row0, q.n, q.len));
+    raw = paged_seq(p.b, s, false);
+    mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
     total += mine;
   }
   total = uniform(wave_sum_int(total) * p.b.Hkv);
@@ -372,8 +374,8 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
       if (p.b.n_seqs > 64) {
         mine = 0;
         if (s0 + lane < p.b.n_seqs) {
-          const PagedSeq q = paged_seq(p.b, s0 + lane, false);
-          mine = step_chunks<KC>(step_seq(p, q.row0, q.n, q.len));
+          raw = paged_seq(p.b, s0 + lane, false);
+          mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
         }
       }
       incl = mine;
@@ -388,13 +390,13 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
         ld.s = uniform(s0 + at);
         before = uniform(before + __shfl(incl - mine, at, 64));
         mine = uniform(__shfl(mine, at, 64));
+        ld.q = step_seq(p, uniform(__shfl(raw.row0, at, 64)), uniform(__shfl(raw.n, at, 64)), uniform(__shfl(raw.len, at, 64)));
         break;
       }
       before += uniform(__shfl(incl, 63, 64));
       s0 += 64;
       if (s0 >= p.b.n_seqs) return;  // not reached: begin < total
     }
-    ld.q = step_seq_at(p, ld.s);
     const int off = begin - before * p.b.Hkv;
     ld.h = uniform(off / mine);
     ld.c = uniform(ld.q.lo / KC + off % mine);
@@ -545,37 +547,42 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
   if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
 
-// Joins the parts of one (row, query head): out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m the
-// largest m_i. Also what the step kernel has no chunk for: zeros for rows that see nothing, and the
-// report of bounds that are out of range. Every workgroup finds its parts from the lengths, as the
-// step kernel found its runs; the parts are taken in their order, so results repeat bit for bit.
+// Joins the parts of a row's query heads of one kv head: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,
+// m the largest m_i. Also what the step kernel has no chunk for: zeros for rows that see nothing, and the
+// report of bounds that are out of range. Every workgroup finds its parts from the lengths, as the step
+// kernel found its runs; the parts are taken in a fixed order, so results repeat bit for bit.
 template <typename T, int D, int KC, int PBQ>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads of a part, parts at a time
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads of a part, groups of them
+  constexpr int kPhases = 4, kHeads = kGroups / kPhases;  // a head's parts go round four groups
   __shared__ int sums[4][2];
+  __shared__ int found;
   __shared__ f32x4 acc[kGroups][kLanes];
-  __shared__ float lsum[kGroups];
+  __shared__ float2 accml[kGroups];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x / p.b.Hq, head = blockIdx.x - t * p.b.Hq, g = p.b.Hq / p.b.Hkv;
-  const int sq = seq_of_row(p.b, t, lane);
-  if (sq >= p.b.n_seqs) return;
-  const PagedSeq raw = paged_seq(p.b, sq, head == 0 && tid == 0);
-  const StepSeq q = step_seq(p, raw.row0, raw.n, raw.len);
-  const int i = t - raw.row0;
-  if (i < 0 || i >= raw.n) return;
-  if (head == 0 && i == 0 && wave == 0 && p.shared > 0) check_shared(p.b, sq, raw, p.shared, lane);
-  if (i >= q.n) {
-    if (tid == 0) latch(p.b.status, kBadSequence);
-    return;
-  }
-  T* orow = (T*)p.out + (int64_t)t * p.ld_out + head * D;
-  const int chunks = step_chunks<KC>(q);
-  int all = 0, before = 0;
+  const int t = blockIdx.x / p.b.Hkv, hk = blockIdx.x - t * p.b.Hkv, g = p.b.Hq / p.b.Hkv;
+  const bool reports = blockIdx.x == 0 && blockIdx.y == 0;
+  // the row's sequence, and the chunks of all and of those before it
+  if (tid == 0) found = -1;
+  __syncthreads();
+  int all = 0, mine = 0;
   for (int s = tid; s < p.b.n_seqs; s += 256) {
-    const PagedSeq x = paged_seq(p.b, s, false);
-    const int c = step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
-    all += c;
-    before += s < sq ? c : 0;
+    const PagedSeq x = paged_seq(p.b, s, reports);
+    mine = step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
+    all += mine;
+    if (x.row0 <= t && t < x.row0 + x.n) atomicMax(&found, s);
+  }
+  __syncthreads();
+  const int sq = found;
+  if (sq < 0) return;
+  int before = 0;
+  if (p.b.n_seqs <= 256) {
+    before = tid < sq ? mine : 0;
+  } else {
+    for (int s = tid; s < sq; s += 256) {
+      const PagedSeq x = paged_seq(p.b, s, false);
+      before += step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
+    }
   }
   all = wave_sum_int(all);
   before = wave_sum_int(before);
@@ -583,56 +590,68 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
     sums[wave][0] = all;
     sums[wave][1] = before;
   }
+  const PagedSeq raw = paged_seq(p.b, sq, false);
+  const StepSeq q = step_seq(p, raw.row0, raw.n, raw.len);
+  const int i = t - raw.row0;
+  if (hk == 0 && blockIdx.y == 0 && i == 0 && wave == 0 && p.shared > 0) check_shared(p.b, sq, raw, p.shared, lane);
+  if (i >= q.n) {
+    if (tid == 0) latch(p.b.status, kBadSequence);
+    return;
+  }
   __syncthreads();
   all = (sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0]) * p.b.Hkv;
   before = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
-  if (chunks == 0 && p.skip == 0) {
-    if (tid < kLanes) store_run(orow + 4 * tid, f32x4{0.f, 0.f, 0.f, 0.f});
-    return;
-  }
+  const int chunks = step_chunks<KC>(q);
   int own = 0, wa = 0;  // parts of the row's own chunks
   bool at_start = false;
   if (chunks > 0) {
     const int per = (int)(((uint32_t)all + p.workers - 1) / (uint32_t)p.workers);
-    const int a = before * p.b.Hkv + (head / g) * chunks;
+    const int a = before * p.b.Hkv + hk * chunks;
     wa = a / per;
     own = (a + chunks - 1) / per - wa + 1;
     at_start = a == wa * per;
   }
   if (own == 1 && p.skip == 0) return;  // finished by the step kernel
-  const int rows = p.max_q * g, row = i * g + head % g, parts = own + (p.skip > 0 ? p.splits : 0);
-  // part k: the row's own chunks', then the prefix's
-  auto slot = [&](int k) -> int64_t {
-    if (k >= own) {
-      const int r = t * g + head % g;
-      return ((int64_t)((head / g) * p.splits + k - own) * p.row_blocks + r / PBQ) * PBQ + r % PBQ;
-    }
-    if (own == 1) return (int64_t)2 * p.workers * rows + (int64_t)t * p.b.Hq + head;
-    return (int64_t)(2 * (wa + k) + (k > 0 || at_start ? 0 : 1)) * rows + row;
-  };
-  float m = -INFINITY;
-  for (int k = lane; k < parts; k += 64) m = fmaxf(m, (k < own ? p.part_ml : p.pre_ml)[slot(k)].x);
-  m = wave_max(m);
-  if (m == -INFINITY) m = 0.f;
+  const int rows = p.max_q * g, parts = own + (p.skip > 0 ? p.splits : 0);
   const int grp = tid / kLanes, at = tid % kLanes;
+  const int h = blockIdx.y * kHeads + grp / kPhases, phase = grp % kPhases;
+  const int row = i * g + h, prow = t * g + h;
+  const int64_t whole = (int64_t)2 * p.workers * rows + (int64_t)t * p.b.Hq + hk * g + h;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int k = grp; k < parts; k += kGroups) {
-    const int64_t s = slot(k);
-    const float2 ml = (k < own ? p.part_ml : p.pre_ml)[s];
-    const float e = __builtin_amdgcn_exp2f(ml.x - m);
-    l += e * ml.y;
-    o += e * *reinterpret_cast<const f32x4*>((k < own ? p.part_o : p.pre_o) + s * D + 4 * at);
+  float m = -INFINITY, l = 0.f;
+  if (h < g) {
+#pragma unroll 4
+    for (int k = phase; k < parts; k += kPhases) {
+      const bool pre = k >= own;  // the prefix's
+      const int64_t mine_at = own == 1 ? whole : (int64_t)(2 * (wa + k) + (k > 0 || at_start ? 0 : 1)) * rows + row;
+      const int64_t pre_at = ((int64_t)(hk * p.splits + k - own) * p.row_blocks + prow / PBQ) * PBQ + prow % PBQ;
+      const int64_t s = pre ? pre_at : mine_at;
+      const float2 ml = (pre ? p.pre_ml : p.part_ml)[s];
+      const f32x4 x = *reinterpret_cast<const f32x4*>((pre ? p.pre_o : p.part_o) + s * D + 4 * at);
+      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float e0 = __builtin_amdgcn_exp2f(m - ref), e1 = __builtin_amdgcn_exp2f(ml.x - ref);
+      l = e0 * l + e1 * ml.y;
+      o = e0 * o + e1 * x;
+      m = m_new;
+    }
   }
   acc[grp][at] = o;
-  if (at == 0) lsum[grp] = l;
+  if (at == 0) accml[grp] = make_float2(m, l);
   __syncthreads();
-  if (tid < kLanes) {
-    for (int k = 1; k < kGroups; ++k) {
-      o += acc[k][tid];
-      l += lsum[k];
+  if (phase == 0 && h < g) {
+    float top = m;
+#pragma unroll
+    for (int k = 1; k < kPhases; ++k) top = fmaxf(top, accml[grp + k].x);
+    const float ref = top == -INFINITY ? 0.f : top, e0 = __builtin_amdgcn_exp2f(m - ref);
+    l *= e0;
+    o *= e0;
+#pragma unroll
+    for (int k = 1; k < kPhases; ++k) {
+      const float e = __builtin_amdgcn_exp2f(accml[grp + k].x - ref);
+      l += e * accml[grp + k].y;
+      o += e * acc[grp + k][at];
     }
-    store_run(orow + 4 * tid, o * (l > 0.f ? 1.f / l : 0.f));
+    store_run((T*)p.out + (int64_t)t * p.ld_out + (hk * g + h) * D + 4 * at, o * (l > 0.f ? 1.f / l : 0.f));
   }
 }
 
@@ -643,12 +662,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 // and values) against chunks of KC positions in LDS, double-buffered by direct loads. A plan made on the
 // device lists the blocks of all sequences and the chunks that each sees; per kv head they are one line,
 // the lines one after another, cut into equal runs for as many workgroups as are resident: neither
-// unequal lengths nor the causal triangle leave a workgroup idle. A block cut by a run's border leaves
-// parts, which a third launch joins.
+// unequal lengths nor the causal triangle leave a workgroup idle. A block takes kTileStart places on the
+// line before its chunks, for what starting and ending it costs (without them the run with the many short
+// blocks of a prompt's first rows took 202 us beside 118 of the others, four prompts of 2048 at D 256). A
+// block cut by a run's border leaves parts, which a third launch joins.
+constexpr int kTileStart = 2;
+
 template <int BQ, int KC>
 __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* total) {
+  constexpr int kKeep = 2048;
   __shared__ int wsum[16];
   __shared__ int carry;
+  __shared__ int keep[kKeep];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.b.Hq / p.b.Hkv;
   // inclusive sum over the workgroup plus what went before; all threads call it
   auto scan = [&](int x) {
@@ -672,8 +697,8 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
   };
   if (tid == 0) carry = 0;
   __syncthreads();
-  // the first block of each sequence goes where it belongs in the list; the rest follow from it
-  int* first = total + 1;  // [n_seqs + 1]
+  // each sequence's first block in the list; all others follow from them
+  int* first = p.b.n_seqs <= kKeep ? keep : total + 2;
   for (int s0 = 0; s0 < p.b.n_seqs; s0 += 1024) {
     const int s = s0 + tid;
     int n = 0;
@@ -686,16 +711,13 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
     if (s < p.b.n_seqs) first[s] = end - n;
   }
   const int tiles = min(carry, p.most_tiles);
-  __syncthreads();
-  if (tid == 0) {
-    first[p.b.n_seqs] = tiles;
-    carry = 0;
-  }
   __threadfence_block();
+  __syncthreads();
+  if (tid == 0) carry = 0;
   __syncthreads();
   for (int t0 = 0; t0 < tiles; t0 += 1024) {
     const int t = t0 + tid;
-    PagedTile x = {0, 0, 0, 0, 0};
+    PagedTile x = {};
     if (t < tiles) {
       int lo = 0, hi = p.b.n_seqs;  // the last s with first[s] <= t
       while (hi - lo > 1) {
@@ -704,24 +726,29 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
         else hi = mid;
       }
       const PagedSeq q = paged_seq(p.b, lo, false);
-      const int n = min(q.n, p.max_q), base = q.len - q.n;
       x.seq = lo;
       x.row = (t - first[lo]) * BQ;
-      const int a = max(0, p.window > 0 ? base + x.row / g - p.window + 1 : 0);
-      const int e = base + (min(x.row + BQ, n * g) - 1) / g + 1;
+      x.row0 = q.row0;
+      x.base = q.len - q.n;
+      x.n = min(q.n, p.max_q) * g;
+      const int a = max(0, p.window > 0 ? x.base + x.row / g - p.window + 1 : 0);
+      const int e = x.base + (min(x.row + BQ, x.n) - 1) / g + 1;
       x.chunk0 = a / KC;
       x.chunks = e > a ? (e + KC - 1) / KC - x.chunk0 : 0;
     }
-    const int end = scan(x.chunks);
-    x.at = end - x.chunks;
+    const int len = x.chunks > 0 ? x.chunks + kTileStart : 0;
+    x.at = scan(len) - len + kTileStart;
     if (t < tiles) p.tiles[t] = x;
   }
-  if (tid == 0) *total = carry;
+  if (tid == 0) {
+    total[0] = carry;
+    total[1] = tiles;
+  }
   if (p.shared > 0)
     for (int s = wave; s < p.b.n_seqs; s += 16) check_shared(p.b, s, paged_seq(p.b, s, false), p.shared, lane);
 }
 
-// Where on the lines a worker's run begins and ends: total chunks of a line, as equal runs as can be.
+// The length of the runs, all places of the kv heads' lines in as equal ones as can be.
 __device__ __forceinline__ int tile_run(const PagedAttn& p, int line) {
   return (int)(((uint32_t)line * p.b.Hkv + p.workers - 1) / (uint32_t)p.workers);
 }
@@ -739,96 +766,141 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   const int g = p.b.Hq / p.b.Hkv;
   // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
   const int w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
-  int line = 1, tiles = 0, at = w, stop = min(w + 1, p.b.Hkv * p.splits * p.row_blocks);
-  if constexpr (!PREFIX) {
-    line = total[0];
-    tiles = total[1 + p.b.n_seqs];
-    const int per = tile_run(p, line);
-    at = w * per;
-    stop = min(line * p.b.Hkv, at + per);
-  }
   const uint32_t ring0 = lds_offset(ring);
-  bool first_item = true, bad = false;
-  while (at < stop) {
-    int h, c0, count, chunks, seq_row, base, n, row0, hi_pos, lo_pos;
-    const int32_t* pages = p.b.table;
-    if constexpr (PREFIX) {
-      h = at / (p.splits * p.row_blocks);
-      const int split = at / p.row_blocks % p.splits, all = (p.skip + KC - 1) / KC;
-      c0 = (int)((int64_t)split * all / p.splits);
-      count = (int)((int64_t)(split + 1) * all / p.splits) - c0;
-      chunks = seq_row = 0;
-      row0 = at % p.row_blocks * BQ;
-      n = p.b.n_rows * g;
-      base = p.skip - 1;
-      hi_pos = p.skip;
-      lo_pos = 0;
-    } else {
-      h = at / line;
-      const int off = at - h * line;
-      int lo = 0, hi = tiles;  // the last tile that starts at or before off: it has chunks
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.tiles[mid].at <= off) lo = mid;
-        else hi = mid;
-      }
-      const PagedTile x = p.tiles[lo];
-      c0 = uniform(x.chunk0 + off - x.at);
-      count = uniform(min(x.at + x.chunks - off, stop - at));
-      chunks = uniform(x.chunks);
-      const int seq = uniform(x.seq);
-      const PagedSeq q = paged_seq(p.b, seq, false);
-      seq_row = uniform(q.row0);
-      n = uniform(min(q.n, p.max_q) * g);
-      base = uniform(q.len - q.n);
-      row0 = uniform(x.row);
-      hi_pos = base + (min(row0 + BQ, n) - 1) / g + 1;
-      lo_pos = max(0, p.window > 0 ? base + row0 / g - p.window + 1 : 0);
-      pages += (int64_t)seq * p.b.ld_table;
-    }
-    // the position of the block's row r
-    auto position = [&](int r) { return PREFIX ? base : base + r / g; };
 
-    // the wave's blocks of 16 positions in every chunk (keys' blocks, then values'), their pages looked up a
-    // chunk ahead; one that no row of the block of rows sees is read from page 0 (masked, and zeroed)
-    constexpr int kMine = (2 * KT + NW - 1) / NW;
-    int id[kMine];
-    auto look_up = [&](int c) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int pos = c * KC + 16 * ((i * NW + wave) % KT);
-        id[i] = uniform(const_ints(pages)[min(pos >> p.b.page_shift, p.b.cols - 1)]);
+  // the part of a block's chunks that the run holds: chunks c0 .. c0 + count - 1 of kv head h
+  struct Item {
+    int h, c0, count, chunks, seq, row0, base, n, row, hi_pos, lo_pos;
+  };
+  int at = w, stop = min(w + 1, p.b.Hkv * p.splits * p.row_blocks), line = 1, tiles = 0, tile = 0, head = 0;
+  typedef const __attribute__((address_space(4))) PagedTile* ConstTiles;
+  ConstTiles list = (ConstTiles)(uintptr_t)p.tiles;
+  // goes to the first block from (head, tile) on that sees anything, and `at` to its first chunk
+  auto seek = [&]() {
+    if constexpr (!PREFIX) {
+      while (true) {
+        if (tile == tiles) {
+          tile = 0;
+          ++head;
+        }
+        if (head == p.b.Hkv || uniform(list[tile].chunks) > 0) break;
+        ++tile;
       }
-    };
-    auto issue = [&](int c, int stage) {
+      at = head == p.b.Hkv ? stop : head * line + uniform(list[tile].at);
+    }
+  };
+  // the item there, of which the run holds the chunks from place `begin` on; goes on to the next one
+  auto item = [&](int begin) {
+    Item x;
+    if constexpr (PREFIX) {
+      x.h = at / (p.splits * p.row_blocks);
+      const int split = at / p.row_blocks % p.splits, all = (p.skip + KC - 1) / KC;
+      x.c0 = (int)((int64_t)split * all / p.splits);
+      x.count = (int)((int64_t)(split + 1) * all / p.splits) - x.c0;
+      x.chunks = x.seq = x.row0 = x.lo_pos = 0;
+      x.row = at % p.row_blocks * BQ;
+      x.n = p.b.n_rows * g;
+      x.base = p.skip - 1;
+      x.hi_pos = p.skip;
+      at += 1;
+    } else {
+      begin = max(begin, at);
+      x.h = head;
+      x.chunks = uniform(list[tile].chunks);
+      x.c0 = uniform(list[tile].chunk0) + begin - at;
+      x.count = min(at + x.chunks, stop) - begin;
+      x.seq = uniform(list[tile].seq);
+      x.row0 = uniform(list[tile].row0);
+      x.base = uniform(list[tile].base);
+      x.n = uniform(list[tile].n);
+      x.row = uniform(list[tile].row);
+      x.hi_pos = x.base + (min(x.row + BQ, x.n) - 1) / g + 1;
+      x.lo_pos = max(0, p.window > 0 ? x.base + x.row / g - p.window + 1 : 0);
+      ++tile;
+      seek();
+    }
+    return x;
+  };
+  int begin = at;
+  if constexpr (!PREFIX) {
+    ConstInts tot = const_ints(total);
+    line = uniform(tot[0]);
+    tiles = uniform(tot[1]);
+    const int per = tile_run(p, line);
+    begin = w * per;
+    stop = min(line * p.b.Hkv, begin + per);
+    if (begin >= stop) return;
+    // the block in which the run begins: the last whose places start at or before it
+    head = begin / line;
+    const int off = begin - head * line;
+    int* count = (int*)ring;
+    int mine = 0;
+    for (int i = tid; i < tiles; i += 64 * NW) mine += p.tiles[i].at - kTileStart <= off ? 1 : 0;
+    mine = wave_sum_int(mine);
+    if (lane == 0) count[wave] = mine;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) tile += count[i];
+    tile = uniform(tile) - 1;
+    __syncthreads();
+    seek();
+  }
+  if (at >= stop) return;
+
+  // the wave's blocks of 16 positions in every chunk (keys' blocks, then values'), their pages looked up a
+  // chunk ahead; one that no row of the block of rows sees is read from page 0 (masked, and zeroed)
+  constexpr int kMine = (2 * KT + NW - 1) / NW;
+  int id[kMine];
+  bool bad = false;
+  auto look_up = [&](const Item& x, int c) {
+    ConstInts pages = const_ints(p.b.table) + (int64_t)x.seq * p.b.ld_table;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int blk = i * NW + wave;
-        if (2 * KT % NW != 0 && blk >= 2 * KT) break;
-        const int j = blk % KT, pos = c * KC + 16 * j;
-        const bool use = pos < hi_pos && pos + 16 > lo_pos, ok = (uint32_t)id[i] < (uint32_t)p.b.n_pages;
-        bad |= use && !ok;
-        const int slot = pos & ((1 << p.b.page_shift) - 1);
-        const int64_t from = ((((int64_t)(use && ok ? id[i] : 0) * p.b.Hkv + h) << p.b.page_shift) + slot) * R::kBytes;
-        const int lds = (int)ring0 + stage * 2 * kHalf + (blk / KT) * kHalf + j * 16 * R::kBytes;
-        if (blk < KT) load_block16<T, D, true>(uniform((const unsigned char*)p.k + from), uniform(lds), lane);
-        else load_block16<T, D, false>(uniform((const unsigned char*)p.v + from), uniform(lds), lane);
-      }
-    };
-    look_up(c0);
-    issue(c0, 0);
-    if (count > 1) look_up(c0 + 1);
+    for (int i = 0; i < kMine; ++i) {
+      const int pos = c * KC + 16 * ((i * NW + wave) % KT);
+      id[i] = uniform(pages[min(pos >> p.b.page_shift, p.b.cols - 1)]);
+    }
+  };
+  auto issue = [&](const Item& x, int c, int stage) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int blk = i * NW + wave;
+      if (2 * KT % NW != 0 && blk >= 2 * KT) break;
+      const int j = blk % KT, pos = c * KC + 16 * j;
+      const bool use = pos < x.hi_pos && pos + 16 > x.lo_pos, ok = (uint32_t)id[i] < (uint32_t)p.b.n_pages;
+      bad |= use && !ok;
+      const int slot = pos & ((1 << p.b.page_shift) - 1);
+      const int64_t from = ((((int64_t)(use && ok ? id[i] : 0) * p.b.Hkv + x.h) << p.b.page_shift) + slot) * R::kBytes;
+      const int lds = (int)ring0 + stage * 2 * kHalf + (blk / KT) * kHalf + j * 16 * R::kBytes;
+      if (blk < KT) load_block16<T, D, true>(uniform((const unsigned char*)p.k + from), uniform(lds), lane);
+      else load_block16<T, D, false>(uniform((const unsigned char*)p.v + from), uniform(lds), lane);
+    }
+  };
+
+  // chunks follow one another through the two buffers, across the items' borders too
+  Item x = item(begin);
+  int stage = 0;
+  bool first_item = true;
+  look_up(x, x.c0);
+  issue(x, x.c0, 0);
+  while (true) {
+    const bool more = at < stop;
+    Item next = x;
+    if (more) next = item(at);
+    if (x.count > 1) look_up(x, x.c0 + 1);
+    else if (more) look_up(next, next.c0);
+    const int h = x.h, n = x.n;
+    // the position of the block's row r
+    auto position = [&](int r) { return PREFIX ? x.base : x.base + r / g; };
 
     // this wave's rows
     uint4 qf[RG * M::KS];
     int pos_r[RG], lo_r[RG];
     f32x4 o[RG * M::DT];
     float m_run[RG], l_part[RG];
-    const int wrow = row0 + wave * 16 * RG;
+    const int wrow = x.row + wave * 16 * RG;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
       const int r = min(wrow + 16 * i + fr, n - 1), token = r / g;
-      const T* qr = (const T*)p.q + (int64_t)(seq_row + token) * p.ld_q + (h * g + r - token * g) * D;
+      const T* qr = (const T*)p.q + (int64_t)(x.row0 + token) * p.ld_q + (h * g + r - token * g) * D;
 #pragma unroll
       for (int ks = 0; ks < M::KS; ++ks)
         qf[i * M::KS + ks] = *reinterpret_cast<const uint4*>(qr + (4 * ks + fg) * R::kVec);
@@ -848,18 +920,21 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     const int lo_first = p.window > 0 ? max(0, pos_first - p.window + 1) : 0;
     const bool rows_here = wrow < n;
 
-    for (int ch = 0; ch < count; ++ch) {
-      const int k0 = (c0 + ch) * KC;
-      const unsigned char* keys = ring[ch & 1];
-      unsigned char* vals = ring[ch & 1] + kHalf;
+    for (int ch = 0; ch < x.count; ++ch) {
+      const int k0 = (x.c0 + ch) * KC;
+      const unsigned char* keys = ring[stage];
+      unsigned char* vals = ring[stage] + kHalf;
+      stage ^= 1;
       dma_stage_sync<0>();  // this chunk has landed, and every wave is done with the other buffer
-      if (ch + 1 < count) issue(c0 + ch + 1, (ch + 1) & 1);
-      if (ch + 2 < count) look_up(c0 + ch + 2);
-      if (k0 < lo_pos || k0 + KC > hi_pos) {
+      if (ch + 1 < x.count) issue(x, x.c0 + ch + 1, stage);
+      else if (more) issue(next, next.c0, stage);
+      if (ch + 2 < x.count) look_up(x, x.c0 + ch + 2);
+      else if (ch + 2 == x.count && more) look_up(next, next.c0);
+      if (k0 < x.lo_pos || k0 + KC > x.hi_pos) {
         // positions that no row of the block sees may hold anything, and 0 times a NaN would be one
         for (int y = tid; y < KC * R::kPieces; y += 64 * NW) {
           const int key = k0 + y / R::kPieces;
-          if (key < lo_pos || key >= hi_pos) *reinterpret_cast<uint4*>(vals + y * 16) = make_uint4(0, 0, 0, 0);
+          if (key < x.lo_pos || key >= x.hi_pos) *reinterpret_cast<uint4*>(vals + y * 16) = make_uint4(0, 0, 0, 0);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       }
@@ -903,7 +978,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       }
       M::template values<KT, RG>(vals, s, o, lane);
     }
-    const bool all = count == chunks;
+    const bool all = x.count == x.chunks;
     const int64_t slot = (PREFIX ? (int64_t)w : (int64_t)2 * w + (first_item ? 0 : 1)) * BQ;
     float* part_o = PREFIX ? p.pre_o : p.part_o;
     float2* part_ml = PREFIX ? p.pre_ml : p.part_ml;
@@ -914,18 +989,18 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       const int r = wrow + 16 * i + fr, token = r / g;
       if (r >= n) continue;
       if (!PREFIX && all) {
-        T* orow = (T*)p.out + (int64_t)(seq_row + token) * p.ld_out + (h * g + r - token * g) * D;
+        T* orow = (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
         const float inv = l > 0.f ? 1.f / l : 0.f;
         M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(orow + d, y * inv); });
       } else {
-        const int64_t at_row = slot + r - row0;
+        const int64_t at_row = slot + r - x.row;
         M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(part_o + at_row * D + d, y); });
         if (fg == 0) part_ml[at_row] = make_float2(m_run[i], l);
       }
     }
     first_item = false;
-    at += count;
-    if (at < stop) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // both buffers are free
+    if (!more) break;
+    x = next;
   }
   if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
@@ -936,21 +1011,22 @@ template <typename T, int D, int BQ>
 __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const int* total) {
   constexpr int kLanes = D / 4, kRows = 256 / kLanes;
   const int tid = threadIdx.x, g = p.b.Hq / p.b.Hkv;
-  const int line = total[0], tiles = total[1 + p.b.n_seqs];
+  const int line = total[0], tiles = total[1];
   const int t = blockIdx.x, h = blockIdx.y;
   if (t >= tiles) return;
   const PagedTile x = p.tiles[t];
+  // the workers' runs that its chunks lie in; in each but the first the block is the first item, in that one
+  // only if the run begins where no earlier block has chunks
   const int per = tile_run(p, line), a = h * line + x.at;
   const int wa = x.chunks > 0 ? a / per : 0, parts = x.chunks > 0 ? (a + x.chunks - 1) / per - wa + 1 : 0;
   if (parts == 1) return;
-  const PagedSeq q = paged_seq(p.b, x.seq, false);
-  const int n = min(q.n, p.max_q) * g, last = min(x.row + (int)(blockIdx.z + 1) * 16, n);
+  const int last = min(x.row + (int)(blockIdx.z + 1) * 16, x.n);
   const int lane = tid % kLanes;
   for (int r = x.row + blockIdx.z * 16 + tid / kLanes; r < last; r += kRows) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f, m = -INFINITY;
     auto slot = [&](int k) -> int64_t {
-      return ((int64_t)2 * (wa + k) + (k > 0 || a == wa * per ? 0 : 1)) * BQ + r - x.row;
+      return ((int64_t)2 * (wa + k) + (k > 0 || wa * per >= a - kTileStart ? 0 : 1)) * BQ + r - x.row;
     };
     for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[slot(k)].x);
     if (m == -INFINITY) m = 0.f;
@@ -962,7 +1038,7 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const
       o += e * *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * lane);
     }
     const int token = r / g;
-    T* orow = (T*)p.out + (int64_t)(q.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
+    T* orow = (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
     store_run(orow + 4 * lane, o * (l > 0.f ? 1.f / l : 0.f));
   }
 }
@@ -1032,7 +1108,8 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   }
   if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
   else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
-  paged_join_kernel<T, D, S::KC, P::BQ><<<(unsigned)heads, 256, 0, ctx->stream>>>(p);
+  const dim3 join((unsigned)((int64_t)p.b.n_rows * p.b.Hkv), (unsigned)((g + 256 / D - 1) / (256 / D)));
+  paged_join_kernel<T, D, S::KC, P::BQ><<<join, 256, 0, ctx->stream>>>(p);
   return TL_OK;
 }
 
@@ -1041,7 +1118,7 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   using S = TileShape<T, D>;
   const int64_t g = p.b.Hq / p.b.Hkv;
   const int64_t most = std::min<int64_t>(p.b.n_seqs, p.b.n_rows) + (int64_t)p.b.n_rows * g / S::BQ;
-  const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
+  const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC + kTileStart);
   TL_REQUIRE(line * p.b.Hkv < (1LL << 30), "batch too large: row blocks x kv heads x table positions");
   TL_REQUIRE(p.b.Hkv <= 65535, "more than 65535 kv heads");
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
