@@ -305,11 +305,12 @@ def geglu_ffn(x, wg, wu, wd, activation="gelu", rnd=None):
 
 
 def mqa(x, wqkv, wo, num_heads, num_kv_heads, head_dim, pos0=0, rope_base=10000.0,
-        past_k=None, past_v=None, rnd=None, use_rope=True):
+        past_k=None, past_v=None, rnd=None, use_rope=True, softcap=0.0, window=0):
     """Multi-/grouped-query causal attention with rotate-half RoPE (Shazeer 2019; Ainslie
     et al. 2023; Su et al. 2021). wqkv [C, (Hq + 2 Hkv) D] with columns [Q | K | V]; query
     head h reads key/value head h // (Hq / Hkv). x holds positions pos0 .. pos0 + T - 1;
     past_k/past_v [B, Hkv, pos0, D] are the rotated keys and values of earlier positions.
+    softcap c > 0 caps scores as c tanh(s / c); window w > 0 hides keys at or before p - w.
     Returns (y, k_all, v_all) with k_all/v_all [B, Hkv, pos0 + T, D]."""
     r = rnd or (lambda a: a)
     x = np.asarray(x, dtype=F32)
@@ -333,7 +334,12 @@ def mqa(x, wqkv, wo, num_heads, num_kv_heads, head_dim, pos0=0, rope_base=10000.
     vv = np.repeat(v, g, axis=1)
     s = (q @ kk.transpose(0, 1, 3, 2)) / F32(D ** 0.5)
     qpos = pos0 + np.arange(T)[:, None]
-    s = np.where(np.arange(Tk)[None, :] <= qpos, s, F32(-1e9)).astype(F32)
+    if softcap:
+        s = F32(softcap) * np.tanh(s / F32(softcap))
+    seen = np.arange(Tk)[None, :] <= qpos
+    if window:
+        seen &= np.arange(Tk)[None, :] > qpos - window
+    s = np.where(seen, s, F32(-1e9)).astype(F32)
     s = s - np.max(s, axis=-1, keepdims=True)
     e = np.exp(s)
     p = e / np.sum(e, axis=-1, keepdims=True)
@@ -374,12 +380,16 @@ def gemma_forward(ids, params, cfg, bf16=False, pos0=0, cache=None):
     r = rnd or (lambda a: a)
     ids = np.asarray(ids)
     C = cfg["d"]
+    windows = cfg.get("window", 0)
+    if np.ndim(windows) == 0:
+        windows = [windows] * cfg["layers"]
     x = r(params["table"][ids] * np.sqrt(F32(C)))
     for l in range(cfg["layers"]):
         past = cache.get(l) if cache is not None else None
         h, k, v = mqa(r(rmsnorm(x, params[f"b{l}.g1"], F32(1e-6), 1.0)), params[f"b{l}.wqkv"],
                       params[f"b{l}.wo"], cfg["heads"], cfg["kv_heads"], cfg["head_dim"], pos0,
-                      cfg.get("rope_base", 10000.0), *(past or (None, None)), rnd=rnd)
+                      cfg.get("rope_base", 10000.0), *(past or (None, None)), rnd=rnd,
+                      softcap=cfg.get("softcap", 0.0), window=windows[l])
         if cache is not None:
             cache[l] = (k, v)
         y = r(x + h)

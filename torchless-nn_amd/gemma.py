@@ -10,7 +10,7 @@ import numpy as np
 
 import backend
 import tl_hip as xp
-from layers import DevicePosition, GemmaBlock, KVCache, RMSNorm
+from layers import DevicePosition, GemmaBlock, KVCache, PagedKVCache, RMSNorm
 from transformer_adapters import GPTEmbeddingTable, GPTEmbedBack, ScaledEmbedFront
 
 __all__ = ["GEMMA_2B", "GemmaDecoder", "build_gemma", "seed_gemma"]
@@ -23,16 +23,23 @@ GEMMA_2B = dict(vocab=256000, ctx=8192, layers=18, d=2048, heads=8, kv_heads=1, 
 
 class GemmaDecoder:
     """Layer list [ScaledEmbedFront, GemmaBlock x L, RMSNorm, GPTEmbedBack] over one tied
-    table. forward(ids, cache, pos0) -> logits [B, T, V] (row pitch a multiple of 8)."""
+    table. forward(ids, cache, pos0) -> logits [B, T, V] (row pitch a multiple of 8). cfg may cap
+    scores ("softcap") and let layers look back a "window" of positions only (a number, or one a
+    layer, 0: all); forward_ragged and generate_ragged serve such a model."""
 
     def __init__(self, cfg):
         self.cfg = dict(cfg)
         d = cfg["d"]
         self.table = GPTEmbeddingTable(cfg["vocab"], d)
         self.front = ScaledEmbedFront(self.table, np.sqrt(np.float32(d)))
+        windows = cfg.get("window", 0)
+        windows = [windows] * cfg["layers"] if np.ndim(windows) == 0 else list(windows)
+        if len(windows) != cfg["layers"]:
+            raise ValueError("one window a layer")
         self.blocks = [GemmaBlock(d, cfg["ctx"], cfg["heads"], cfg["kv_heads"], cfg["head_dim"],
-                                  cfg["ffn"], cfg.get("rope_base", 10000.0))
-                       for _ in range(cfg["layers"])]
+                                  cfg["ffn"], cfg.get("rope_base", 10000.0),
+                                  softcap=cfg.get("softcap", 0.0), window=window)
+                       for window in windows]
         self.final_norm = RMSNorm(d, eps=1e-6, gamma_offset=1.0)
         self.back = GPTEmbedBack(self.table)
         self.layers = [self.front, *self.blocks, self.final_norm, self.back]
@@ -89,6 +96,94 @@ class GemmaDecoder:
         logits = self.back.forward(self.final_norm.forward(x))
         xp.argmax(self.last_rows(logits), out=tok)
         return logits
+
+    # -- ragged batches over a paged cache
+    def new_paged_cache(self, n_pages, page_size=64):
+        c = self.cfg
+        return PagedKVCache(c["layers"], n_pages, c["kv_heads"], c["head_dim"], self.dtype, page_size)
+
+    def forward_ragged(self, ids, cache, batch):
+        """Logits [1, S, V] of each sequence's last row for the ids [1, N] of a batch of the paged
+        cache (PagedKVCache.batch), each at its own sequence's position."""
+        x = self.front.forward(ids)
+        for i, blk in enumerate(self.blocks):
+            x = blk.forward(x, cache, i, batch)
+        if batch.max_q > 1:
+            last, C = batch.last_rows(), x.shape[-1]
+            x = xp.embed(last, x.reshape(-1, C), None, last.size, out_shape=(1, last.size, C))
+        return self.back.forward(self.final_norm.forward(x))
+
+    def generate_ragged(self, prompts, n_new, prefix=(), cache=None, page_size=64):
+        """Greedy continuations of prompts (sequences of ids) of unequal lengths, each preceded by
+        `prefix`, as one batch: the prefix's whole pages are computed and kept once for all, the
+        prompts run as ragged rows, and each step's single tokens are one replayed HIP graph. Returns
+        the new ids [len(prompts), n_new] (host int64)."""
+        prefix = [int(i) for i in prefix]
+        prompts = [[int(i) for i in p] for p in prompts]
+        S = len(prompts)
+        if n_new <= 0 or S == 0:
+            return np.zeros((S, max(0, n_new)), np.int64)
+        size = page_size if cache is None else cache.page_size
+        whole = len(prefix) // size * size
+        rests = [prefix[whole:] + p for p in prompts]
+        if min(len(r) for r in rests) == 0:
+            # the last prompt position's logits start an answer, so one must be each sequence's own
+            whole -= size
+            rests = [prefix[max(whole, 0):] + p for p in prompts]
+            if whole < 0 or min(len(r) for r in rests) == 0:
+                raise ValueError("an empty prompt without a prefix")
+        if max(len(r) for r in rests) + whole + n_new - 1 > self.cfg["ctx"]:
+            raise ValueError(f"prompts and {n_new} new tokens exceed the context length {self.cfg['ctx']}")
+        if cache is None:
+            pages = whole // size + sum(-(-(len(r) + n_new) // size) for r in rests)
+            cache = self.new_paged_cache(pages, size)
+        made = []
+        try:
+            root = None
+            if whole:
+                root = cache.add()
+                made.append(root)
+                self.forward_ragged(xp.array(np.asarray([prefix[:whole]], np.int64)), cache,
+                                    cache.batch([root], [whole]))
+            for _ in prompts:
+                made.append(cache.fork(root, whole) if whole else cache.add())
+            seqs = made[len(made) - S:]
+            batch = cache.batch(seqs, [len(r) for r in rests])
+            logits = self.forward_ragged(xp.array(np.asarray([sum(rests, [])], np.int64)), cache, batch)
+            tok, hist = xp.empty((S,), xp.int64), xp.empty((S, n_new), xp.int64)
+            at = xp.array(np.zeros(1, np.int64))
+            xp.argmax(self.last_rows(logits.reshape(S, 1, -1)), out=tok)
+            xp.ids_append(tok, hist, at, 0)
+            if n_new > 1:
+                step = cache.batch(seqs, [1] * S, reserve=n_new - 2)
+                self._ragged_steps(tok, hist, at, cache, step, n_new - 1)
+            return hist.get()
+        finally:
+            for s in made:
+                cache.free(s)
+
+    def _ragged_steps(self, tok, hist, at, cache, batch, n):
+        """n greedy steps of a batch of single tokens: the first eager (packed weights, workspace), the
+        others one captured step replayed."""
+        S = tok.size
+
+        def forward():
+            logits = self.forward_ragged(tok.reshape(1, S), cache, batch)
+            xp.argmax(self.last_rows(logits.reshape(S, 1, -1)), out=tok)
+            xp.i64_add(at, 1)
+            xp.ids_append(tok, hist, at, 0)
+
+        forward()
+        if n > 1:
+            with xp.capture() as g:
+                xp.i32_add(batch.kv_len, 1)
+                forward()
+            try:
+                for _ in range(n - 1):
+                    batch.note_advance(1)
+                    g.launch()
+            finally:
+                g.destroy()
 
     def generate_greedy(self, ids, n_new, cache=None, return_logits=False, graph=True):
         """Prefill `ids` [B, T] into a KV cache, then take `n_new` greedy steps, each feeding

@@ -17,7 +17,7 @@ from network import Network
 from transformer_adapters import GPTEmbeddingTable, GPTEmbedFront, GPTEmbedBack
 
 __all__ = ["build_gpt", "seed_parameters", "GPT_SMALL", "CHAR_GPT", "new_cache",
-           "forward_cached", "generate", "generate_window"]
+           "forward_cached", "forward_ragged", "generate", "generate_window"]
 
 # BASELINE configurations (model shapes only; batch and sequence length are inputs)
 CHAR_GPT = dict(vocab=65, ctx=128, layers=4, d=128, heads=4, act="gelu")
@@ -91,6 +91,26 @@ def forward_cached(net, ids, cache, pos0, last_only=False):
                 B, T, C = x.shape
                 x = xp.DeviceTensor((B, 1, C), x.dtype, pitch=T * x.pitch, buf=x.buf,
                                     offset=x.offset + (T - 1) * x.pitch * x.dtype.itemsize)
+        else:
+            x = layer.forward(x)
+    return x
+
+
+def forward_ragged(net, ids, cache, batch):
+    """The network's layers over the rows of a ragged batch of a PagedKVCache: ids [1, N], each at its
+    own sequence's position, keys and values kept in the cache's pages. Returns the last layer's output
+    (the SoftMax probabilities) for each sequence's last row, [1, S, V]."""
+    n_blocks = sum(isinstance(layer, TransformerBlock) for layer in net.layers)
+    x, i = ids, 0
+    for layer in net.layers:
+        if isinstance(layer, GPTEmbedFront):
+            x = layer.forward(x, pos0=batch)
+        elif isinstance(layer, TransformerBlock):
+            x = layer.forward(x, cache, i, batch)
+            i += 1
+            if i == n_blocks and batch.max_q > 1:
+                last, C = batch.last_rows(), x.shape[-1]
+                x = xp.embed(last, x.reshape(-1, C), None, last.size, out_shape=(1, last.size, C))
         else:
             x = layer.forward(x)
     return x

@@ -28,7 +28,7 @@ from activations import act_code_of
 
 __all__ = ["Dense", "Dropout", "MultiHeadAttention", "TransformerFeedForward", "LayerNorm",
            "RMSNorm", "TransformerBlock", "linear", "KVCache", "MultiQueryAttention",
-           "GeGLUFeedForward", "GemmaBlock", "DevicePosition"]
+           "GeGLUFeedForward", "GemmaBlock", "DevicePosition", "PagedKVCache", "PagedBatch"]
 
 
 def _round_up(n, m):
@@ -217,6 +217,7 @@ class MultiHeadAttention(Layer):
 
     def _forward(self, input, residual, cache=None, layer=0, pos0=0):
         """Returns heads @ W_o + b_o, plus `residual` when given (fused in the epilogue).
+        With a PagedKVCache, pos0 is one of its batches and input the batch's rows [1, N, C].
         With a KVCache (not in the reference, whose generation recomputes the window,
         demo.ipynb:1526-1533), a decoder writes this call's keys and values into the cache
         at positions pos0 .. and attends over positions 0 .. pos0 + T - 1."""
@@ -264,6 +265,8 @@ class MultiHeadAttention(Layer):
         H, D = self.num_heads, self.heads_dim
         if not self.is_decoder:
             raise ValueError("a KV cache serves causal (decoder) attention only")
+        if isinstance(cache, PagedKVCache):
+            return self._forward_paged(input, residual, cache, layer, pos0)
         if pos0 < 0 or pos0 + T > min(cache.capacity, self.context_length):
             raise ValueError(f"positions up to {pos0 + T} exceed the cache ({cache.capacity}) "
                              f"or the context length ({self.context_length})")
@@ -288,6 +291,19 @@ class MultiHeadAttention(Layer):
         out = linear(heads._rows(), self.out_weights, self.out_bias,
                      residual=_residual_rows(residual, B * T, C))
         self.output = out._reshaped((B, T, C), B * T, C)
+        return self.res_dropout.forward(self.output)
+
+    def _forward_paged(self, input, residual, cache, layer, batch):
+        """The rows of a ragged batch, [1, N, C], over a paged cache."""
+        if self.attn_dropout.dropout_rate > 0.0 and not self.attn_dropout.eval_mode:
+            self.attn_dropout.forward(input)  # raises: no dropout sampling at inference
+        H, D = self.num_heads, self.heads_dim
+        qkv = linear(input._rows(), self.qkv_weights, self.qkv_bias)
+        self.query, self.heads_out = _attend_paged(qkv, cache, layer, batch, H, H, D, self.context_length)
+        self.key_t, self.value, self.softmax = cache.k[layer], cache.v[layer], None
+        out = linear(self.heads_out, self.out_weights, self.out_bias,
+                     residual=_residual_rows(residual, input.nrows, input.ncols))
+        self.output = out._reshaped(input.shape, input.nrows, input.ncols)
         return self.res_dropout.forward(self.output)
 
     def _unfused(self, q, k, vt, B, T, C, H, D, dt, divisor):
@@ -504,18 +520,186 @@ class KVCache:
         self.length = 0  # valid positions written so far
 
 
+class PagedBatch:
+    """The rows of some sequences of a PagedKVCache, one sequence after another: what a forward over
+    ragged rows takes in a position's place. On the device (int32): `page_table` [S, pages], `q_start`
+    [S + 1] (rows q_start[s] .. are sequence s's) and `kv_len` [S] (its length with them). `rows` in
+    all, `max_q` of a sequence at most, `shared` leading positions in the same pages for all."""
+
+    def __init__(self, cache, seqs, counts, lengths, limits, shared):
+        self.cache, self.seqs, self.counts, self.lengths = cache, tuple(seqs), tuple(counts), list(lengths)
+        self.rows, self.max_q, self.shared = sum(counts), max(counts, default=1), shared
+        self._limits = limits  # positions that each sequence's pages hold
+        self._starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        table = np.zeros((len(seqs), max([1] + [len(cache.pages[s]) for s in seqs])), np.int32)
+        for i, s in enumerate(seqs):
+            table[i, :len(cache.pages[s])] = cache.pages[s]
+        self.page_table, self.q_start = xp.array(table), xp.array(self._starts)
+        self.kv_len = xp.array(np.asarray(lengths, np.int32))
+        self._positions = self._last = None
+        self._advanced = False
+
+    def pages(self, layer):
+        """The arguments of xp.kv_append and xp.paged_attention that say where keys and values are."""
+        return (self.cache.k[layer], self.cache.v[layer], self.page_table, self.q_start, self.kv_len)
+
+    def positions(self):
+        """The rows' positions, int64 on the device (of the batch as it was made: a step's batch that
+        has advanced has none)."""
+        if self._positions is None:
+            if self._advanced:
+                raise ValueError("the batch has advanced past the positions that it was made for")
+            at = [np.arange(n - r, n) for n, r in zip(self.lengths, self.counts)]
+            self._positions = xp.array(np.concatenate(at).astype(np.int64) if at else np.zeros(0, np.int64))
+        return self._positions
+
+    def last_rows(self):
+        """The last row of each sequence, int64 [S] on the device."""
+        if self._last is None:
+            if min(self.counts, default=1) < 1:
+                raise ValueError("a sequence of the batch has no row")
+            self._last = xp.array((self._starts[1:] - 1).astype(np.int64))
+        return self._last
+
+    def advance(self, n=1):
+        """The same rows n positions later (the next step's tokens), on the device: a captured step
+        replays at the new lengths. The pages must have been reserved (PagedKVCache.batch)."""
+        self.note_advance(n)
+        xp.i32_add(self.kv_len, n)
+
+    def note_advance(self, n=1):
+        """The host's share of advance(), for a replayed graph that holds the device's."""
+        if any(m + n > limit for m, limit in zip(self.lengths, self._limits)):
+            raise ValueError("the sequences' pages end here: make a batch that reserves more")
+        self.lengths = [m + n for m in self.lengths]
+        for s, m in zip(self.seqs, self.lengths):
+            self.cache.lengths[s] = m
+        self._advanced = True
+
+
+class PagedKVCache:
+    """Keys and values of many sequences of unequal lengths in pages of `page_size` positions (a power
+    of two, 16 to 4096): per layer two tensors [n_pages, Hkv, page_size, D]. Sequences take pages as
+    they grow (`batch`), can begin with another's pages (`fork`) and give them back (`free`)."""
+
+    def __init__(self, n_layers, n_pages, n_kv_heads, head_dim, dtype, page_size=64):
+        if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two from 16 to 4096")
+        self.page_size, self.n_pages, self.n_kv_heads, self.head_dim = page_size, n_pages, n_kv_heads, head_dim
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        self.k = [xp.zeros(shape, dtype) for _ in range(n_layers)]
+        self.v = [xp.zeros(shape, dtype) for _ in range(n_layers)]
+        self.pages, self.lengths = {}, {}
+        self._latest = {}  # the last batch made for each sequence: earlier ones do not know its pages
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._users = [0] * n_pages
+        self._next = 0
+        self._angles = {}
+
+    def add(self):
+        """A new, empty sequence."""
+        s = self._next
+        self._next += 1
+        self.pages[s], self.lengths[s] = [], 0
+        return s
+
+    def fork(self, seq, length):
+        """A new sequence that begins with the first `length` positions (whole pages) of `seq`, in the
+        same pages."""
+        if length % self.page_size or not 0 <= length <= self.lengths[seq]:
+            raise ValueError(f"a sequence of {self.lengths[seq]} positions can be forked at whole pages of "
+                             f"{self.page_size}, not at {length}")
+        s = self.add()
+        self.pages[s] = self.pages[seq][:length // self.page_size]
+        self.lengths[s] = length
+        for p in self.pages[s]:
+            self._users[p] += 1
+        return s
+
+    def free(self, seq):
+        """Gives a sequence's pages back (those that no other sequence begins with)."""
+        for p in self.pages.pop(seq):
+            self._users[p] -= 1
+            if not self._users[p]:
+                self._free.append(p)
+        del self.lengths[seq]
+        self._latest.pop(seq, None)
+
+    def batch(self, seqs, counts, reserve=0):
+        """Rows for `counts` new positions of the sequences `seqs`, which grow by them; pages are taken
+        for those and for `reserve` more (PagedBatch.advance)."""
+        seqs, counts = [int(s) for s in seqs], [int(n) for n in counts]
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or min(counts, default=0) < 0 or reserve < 0:
+            raise ValueError("a batch needs different sequences and a count of new positions for each")
+        size = self.page_size
+        lengths = [self.lengths[s] + n for s, n in zip(seqs, counts)]
+        need = [max(0, -(-(n + reserve) // size) - len(self.pages[s])) for s, n in zip(seqs, lengths)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"the cache is full: {sum(need)} pages needed, {len(self._free)} of {self.n_pages} free")
+        # positions that all begin with in the same pages, before any of the new rows
+        shared = 0
+        if len(seqs) > 1:
+            most = min(self.lengths[s] for s in seqs) // size
+            first = self.pages[seqs[0]]
+            while shared < most and all(self.pages[s][shared] == first[shared] for s in seqs):
+                shared += 1
+        for s, n, length in zip(seqs, need, lengths):
+            for _ in range(n):
+                p = self._free.pop()
+                self._users[p] = 1
+                self.pages[s].append(p)
+            self.lengths[s] = length
+        made = PagedBatch(self, seqs, counts, lengths, [len(self.pages[s]) * size for s in seqs], shared * size)
+        for s in seqs:
+            self._latest[s] = made
+        return made
+
+    def angles(self, length, base):
+        """The RoPE table of positions 0 .. length - 1, shared by the layers."""
+        key = (length, base)
+        if key not in self._angles:
+            self._angles[key] = xp.rope_table(length, self.head_dim, base)
+        return self._angles[key]
+
+
+def _attend_paged(qkv, cache, layer, batch, heads, kv_heads, head_dim, context_length, rope_base=None, softcap=0.0,
+                  window=0):
+    """The attention of QKV rows [N, (Hq + 2 Hkv) D] at a batch's positions: keys and values appended to
+    the cache's pages, then the queries over them -> (queries, heads [N, Hq D])."""
+    if not isinstance(batch, PagedBatch) or batch.cache is not cache:
+        raise ValueError("a paged cache is read at one of its own batches (PagedKVCache.batch)")
+    if layer == 0 and not all(cache._latest.get(s) is batch for s in batch.seqs):
+        raise ValueError("the batch is out of date: one of its sequences was freed or has a later batch")
+    if qkv.shape[0] != batch.rows:
+        raise ValueError(f"the batch has {batch.rows} rows, got {qkv.shape[0]}")
+    if max(batch.lengths, default=0) > context_length:
+        raise ValueError(f"positions up to {max(batch.lengths)} exceed the context length {context_length}")
+    if (cache.n_kv_heads, cache.head_dim) != (kv_heads, head_dim):
+        raise ValueError("the cache is for other heads")
+    pages = batch.pages(layer)
+    rope = cache.angles(context_length, rope_base) if rope_base is not None else None
+    q = xp.kv_append(qkv, *pages, n_heads_q=heads, rope=rope)
+    out = xp.paged_attention(q, *pages, max_q=batch.max_q, divisor=float(np.float32(head_dim ** 0.5)), softcap=softcap,
+                             window=window, shared=0 if window else batch.shared)
+    return q, out
+
+
 class MultiQueryAttention(Layer):
     """Multi-/grouped-query causal attention with rotary positions: num_heads query heads
     share num_kv_heads key/value heads (Shazeer 2019, "Fast Transformer Decoding"; Ainslie
     et al. 2023, GQA), rotate-half RoPE on queries and keys (Su et al. 2021), scores divided
     by sqrt(head_dim), no biases. Weights qkv [C, (Hq + 2 Hkv) D] with columns [Q | K | V]
     and out [Hq D, C]. `forward(x, cache, layer, pos0)` writes this call's keys and values
-    into `cache` at positions pos0.. and attends over positions 0 .. pos0 + T - 1."""
+    into `cache` at positions pos0.. and attends over positions 0 .. pos0 + T - 1. With a PagedKVCache
+    and one of its batches in pos0's place, x holds the batch's rows, [1, N, C], each at its own
+    sequence's position; that form alone serves `softcap` c > 0 (scores capped as c tanh(s / c)) and
+    `window` w > 0 (position p sees p - w + 1 .. p)."""
     fused = True
 
     def __init__(self, embedding_dim, context_length, num_heads, num_kv_heads, head_dim,
-                 rope_base=10000.0):
+                 rope_base=10000.0, softcap=0.0, window=0):
         super(MultiQueryAttention, self).__init__()
+        self.softcap, self.window = float(softcap), int(window)
         if num_heads % num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         self.embedding_dim, self.context_length = embedding_dim, context_length
@@ -535,6 +719,10 @@ class MultiQueryAttention(Layer):
     def _forward(self, input, residual, cache=None, layer=0, pos0=0, prenorm=None):
         """`prenorm` (an RMSNorm layer) normalises `input` first (folded into the QKV
         product for a decode step's few rows)."""
+        if isinstance(cache, PagedKVCache):
+            return self._forward_paged(input, residual, cache, layer, pos0, prenorm)
+        if self.softcap or self.window:
+            raise ValueError("a score cap and a window are served from a PagedKVCache")
         if isinstance(pos0, DevicePosition):
             return self._forward_dev(input, residual, cache, layer, pos0, prenorm)
         B, T, C = input.shape
@@ -609,6 +797,17 @@ class MultiQueryAttention(Layer):
         out = linear(heads.reshape(B * T, Hq * D), self.out_weights,
                      residual=(residual.reshape(B * T, C) if residual is not None else None))
         self.output = out.reshape(B, T, C)
+        return self.output
+
+    def _forward_paged(self, input, residual, cache, layer, batch, prenorm=None):
+        self.input = input
+        shape, C = input.shape, input.shape[-1]
+        qkv = linear(input.reshape(-1, C), self.qkv_weights, prenorm=prenorm)
+        _, heads = _attend_paged(qkv, cache, layer, batch, self.num_heads, self.num_kv_heads, self.heads_dim,
+                                 self.context_length, self.rope_base, self.softcap, self.window)
+        out = linear(heads, self.out_weights,
+                     residual=(residual.reshape(-1, C) if residual is not None else None))
+        self.output = out.reshape(*shape)
         return self.output
 
     def _unfused(self, q, k, vt, heads, B, T, Tk, L, Hq, Hkv, D, dt, divisor, pos0):
@@ -713,11 +912,11 @@ class GemmaBlock(Layer):
     run in the GEMM epilogues, as in TransformerBlock."""
 
     def __init__(self, embed_dim, context_length, num_heads, num_kv_heads, head_dim, ffn_hidden,
-                 rope_base=10000.0, eps=1e-6):
+                 rope_base=10000.0, eps=1e-6, softcap=0.0, window=0):
         super(GemmaBlock, self).__init__()
         self.pre_attn_norm = RMSNorm(embed_dim, eps=eps, gamma_offset=1.0)
         self.attn_block = MultiQueryAttention(embed_dim, context_length, num_heads, num_kv_heads,
-                                              head_dim, rope_base)
+                                              head_dim, rope_base, softcap, window)
         self.pre_ffn_norm = RMSNorm(embed_dim, eps=eps, gamma_offset=1.0)
         self.ffn = GeGLUFeedForward(embed_dim, ffn_hidden)
         self.parameters = [*self.pre_attn_norm.parameters, *self.attn_block.parameters,

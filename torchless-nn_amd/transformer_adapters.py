@@ -5,7 +5,7 @@ import numpy as np
 import backend
 import tl_hip as xp
 from utils import Layer
-from layers import _packed_nk, linear
+from layers import PagedBatch, _packed_nk, linear
 
 __all__ = ["VitProjector", "GPTEmbeddingTable", "GPTEmbedFront", "GPTEmbedBack", "VitMLPHead",
            "ScaledEmbedFront"]
@@ -134,7 +134,8 @@ class GPTEmbedFront(Layer):
 
     def forward(self, input, pos0=0):
         """`pos0`: the ids sit at positions pos0 .. (a decode step after a cached prefix;
-        the reference always starts at 0, transformer_adapters.py:146-153)."""
+        the reference always starts at 0, transformer_adapters.py:146-153). A PagedBatch in its
+        place: the ids [1, N] of a ragged batch's rows, each at its own position."""
         if not isinstance(input, xp.DeviceTensor):
             input = xp.array(np.asarray(input))
         self.input = input
@@ -143,6 +144,13 @@ class GPTEmbedFront(Layer):
         if not input.contiguous:
             input = input.copy()
         B, T = input.shape
+        if isinstance(pos0, PagedBatch):
+            if (B, T) != (1, pos0.rows) or max(pos0.lengths, default=0) > self.context_length:
+                raise ValueError(f"expected ids [1, {pos0.rows}] at positions below {self.context_length}")
+            shape = (1, T, self.embedding_table.embed_size)
+            self.output = (xp.embed(input, self.embedding_table.table, None, T, out_shape=shape) +
+                           xp.embed(pos0.positions(), self.pos_embedding_table, None, T, out_shape=shape))
+            return self.output
         if pos0 < 0 or pos0 + T > self.context_length:
             raise ValueError(f"positions up to {pos0 + T} exceed the positional table "
                              f"({self.context_length})")
