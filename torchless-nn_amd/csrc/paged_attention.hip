@@ -13,6 +13,11 @@ struct __attribute__((aligned(32))) PagedTile {
   int seq, row, chunk0, chunks, at, row0, base, n;
 };
 
+// Where a workgroup's run of the lines begins: at `place` of them all, in block `tile` of kv head `head`.
+struct __attribute__((aligned(16))) PagedRun {
+  int place, head, tile, unused;
+};
+
 struct PagedAttn {
   PagedBatch b;
   const void* q;
@@ -34,6 +39,7 @@ struct PagedAttn {
   int splits, row_blocks;
   // the tile kernel's plan: row blocks of the batch, in order; per kv head they are one line of chunks
   PagedTile* tiles;
+  PagedRun* runs;  // [workers + 1]
   int most_tiles;
 };
 
@@ -61,7 +67,7 @@ struct Rows {
   static constexpr int kPerLoad = 64 / kPieces;   // rows that one direct load of a wave covers
   static_assert(kPieces <= 64 && kPerLoad <= 16, "row size");
   __device__ __forceinline__ static int key_swizzle(int row) {
-    return kPieces >= 16 ? row & 15 : (row / (16 / kPieces)) & (kPieces - 1);
+    return kPieces >= 16 ? row & 15 : (row / (16 / (kPieces < 16 ? kPieces : 16))) & (kPieces - 1);
   }
   __device__ __forceinline__ static int value_swizzle(int row) {
     constexpr int kSegs = kPieces / 2;  // of 32 bytes
@@ -665,15 +671,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 // unequal lengths nor the causal triangle leave a workgroup idle. A block takes kTileStart places on the
 // line before its chunks, for what starting and ending it costs (without them the run with the many short
 // blocks of a prompt's first rows took 202 us beside 118 of the others, four prompts of 2048 at D 256). A
-// block cut by a run's border leaves parts, which a third launch joins.
-constexpr int kTileStart = 2;
+// block cut by a run's border leaves parts, which a third launch joins; writing and reading one's outputs in 32
+// bits takes as long as some four chunks, so a border within kTileSnap of a block's edge moves there (but by an
+// eighth of a run at most), and a sequence's long blocks and short ones alternate: two of them together are
+// alike long, and more borders meet edges.
+constexpr int kTileStart = 2, kTileSnap = 4;
 
 template <int BQ, int KC>
 __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* total) {
-  constexpr int kKeep = 2048;
+  constexpr int kKeep = 2048, kKeepTiles = 4096;
   __shared__ int wsum[16];
   __shared__ int carry;
   __shared__ int keep[kKeep];
+  __shared__ int keep_at[kKeepTiles];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.b.Hq / p.b.Hkv;
   // inclusive sum over the workgroup plus what went before; all threads call it
   auto scan = [&](int x) {
@@ -727,10 +737,11 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
       }
       const PagedSeq q = paged_seq(p.b, lo, false);
       x.seq = lo;
-      x.row = (t - first[lo]) * BQ;
       x.row0 = q.row0;
       x.base = q.len - q.n;
       x.n = min(q.n, p.max_q) * g;
+      const int i = t - first[lo], blocks = (x.n + BQ - 1) / BQ;
+      x.row = ((i & 1) ? i >> 1 : blocks - 1 - (i >> 1)) * BQ;
       const int a = max(0, p.window > 0 ? x.base + x.row / g - p.window + 1 : 0);
       const int e = x.base + (min(x.row + BQ, x.n) - 1) / g + 1;
       x.chunk0 = a / KC;
@@ -738,19 +749,48 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
     }
     const int len = x.chunks > 0 ? x.chunks + kTileStart : 0;
     x.at = scan(len) - len + kTileStart;
-    if (t < tiles) p.tiles[t] = x;
+    if (t < tiles) {
+      p.tiles[t] = x;
+      if (tiles <= kKeepTiles) keep_at[t] = x.at;
+    }
   }
+  const int line = carry;
   if (tid == 0) {
-    total[0] = carry;
+    total[0] = line;
     total[1] = tiles;
+  }
+  __threadfence_block();
+  __syncthreads();
+  // the runs
+  const int places = line * p.b.Hkv, per = max((int)(((uint32_t)places + p.workers - 1) / (uint32_t)p.workers), 1);
+  const int snap = min(kTileSnap, per / 8);
+  auto start = [&](int t) { return t == tiles ? line : (tiles <= kKeepTiles ? keep_at[t] : p.tiles[t].at) - kTileStart; };
+  for (int w = tid; w <= p.workers; w += 1024) {
+    PagedRun r = {places, p.b.Hkv, 0, 0};
+    if ((int64_t)w * per < places) {
+      r.head = w * per / line;
+      int off = w * per - r.head * line, lo = 0, hi = tiles;  // the last block that starts at or before off
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start(mid) <= off) lo = mid;
+        else hi = mid;
+      }
+      const int a = start(lo), e = start(lo + 1);
+      if (min(off - a, e - off) <= snap) {
+        if (off - a <= e - off) {
+          off = a;
+        } else {
+          off = e;
+          ++lo;
+        }
+      }
+      r.place = r.head * line + off;
+      r.tile = lo;
+    }
+    p.runs[w] = r;
   }
   if (p.shared > 0)
     for (int s = wave; s < p.b.n_seqs; s += 16) check_shared(p.b, s, paged_seq(p.b, s, false), p.shared, lane);
-}
-
-// The length of the runs, all places of the kv heads' lines in as equal ones as can be.
-__device__ __forceinline__ int tile_run(const PagedAttn& p, int line) {
-  return (int)(((uint32_t)line * p.b.Hkv + p.workers - 1) / (uint32_t)p.workers);
 }
 
 // The same for a shared prefix (PREFIX): all rows of the batch as one sequence that sees positions 0 ..
@@ -826,22 +866,13 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     ConstInts tot = const_ints(total);
     line = uniform(tot[0]);
     tiles = uniform(tot[1]);
-    const int per = tile_run(p, line);
-    begin = w * per;
-    stop = min(line * p.b.Hkv, begin + per);
+    typedef const __attribute__((address_space(4))) PagedRun* ConstRuns;
+    ConstRuns run = (ConstRuns)(uintptr_t)p.runs + w;
+    begin = uniform(run[0].place);
+    stop = uniform(run[1].place);
+    head = uniform(run[0].head);
+    tile = uniform(run[0].tile);
     if (begin >= stop) return;
-    // the block in which the run begins: the last whose places start at or before it
-    head = begin / line;
-    const int off = begin - head * line;
-    int* count = (int*)ring;
-    int mine = 0;
-    for (int i = tid; i < tiles; i += 64 * NW) mine += p.tiles[i].at - kTileStart <= off ? 1 : 0;
-    mine = wave_sum_int(mine);
-    if (lane == 0) count[wave] = mine;
-    __syncthreads();
-    for (int i = 0; i < NW; ++i) tile += count[i];
-    tile = uniform(tile) - 1;
-    __syncthreads();
     seek();
   }
   if (at >= stop) return;
@@ -1005,41 +1036,55 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
 
-// Joins the parts of blocks that a run's border cut, and writes zeros for blocks that see nothing. One
-// workgroup per 16 rows of a (block, kv head).
+// Joins the parts of blocks that runs' borders cut, one workgroup per border and 16 rows (a block that
+// several cut is the first one's), and writes zeros for blocks that see nothing.
 template <typename T, int D, int BQ>
 __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const int* total) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
-  const int tid = threadIdx.x, g = p.b.Hq / p.b.Hkv;
-  const int line = total[0], tiles = total[1];
-  const int t = blockIdx.x, h = blockIdx.y;
-  if (t >= tiles) return;
-  const PagedTile x = p.tiles[t];
-  // the workers' runs that its chunks lie in; in each but the first the block is the first item, in that one
-  // only if the run begins where no earlier block has chunks
-  const int per = tile_run(p, line), a = h * line + x.at;
-  const int wa = x.chunks > 0 ? a / per : 0, parts = x.chunks > 0 ? (a + x.chunks - 1) / per - wa + 1 : 0;
-  if (parts == 1) return;
-  const int last = min(x.row + (int)(blockIdx.z + 1) * 16, x.n);
-  const int lane = tid % kLanes;
-  for (int r = x.row + blockIdx.z * 16 + tid / kLanes; r < last; r += kRows) {
+  constexpr int kLanes = D / 4, kRows = 256 / kLanes < 16 ? 256 / kLanes : 16;
+  const int tid = threadIdx.x, g = p.b.Hq / p.b.Hkv, lane = tid % kLanes;
+  const int line = total[0], tiles = total[1], w = blockIdx.x + 1;
+  auto out_row = [&](const PagedTile& x, int h, int r) {
+    const int token = r / g;
+    return (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D + 4 * lane;
+  };
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    if (p.tiles[t].chunks > 0) continue;
+    const PagedTile x = p.tiles[t];
+    for (int h = 0; h < p.b.Hkv; ++h)
+      for (int i = tid / kLanes; i < 16; i += 256 / kLanes) {
+        const int r = x.row + blockIdx.y * 16 + i;
+        if (r < x.n) store_run(out_row(x, h, r), f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+  }
+  const PagedRun b = p.runs[w];
+  const int before = p.runs[w - 1].place;
+  if (b.place >= line * p.b.Hkv) return;
+  const PagedTile x = p.tiles[b.tile];
+  const int a = b.head * line + x.at, end = a + x.chunks;
+  if (b.place <= a || b.place >= end || before > a) return;
+  // the first part is its run's first item if no earlier block has chunks there; the others are
+  const int64_t part0 = (int64_t)(2 * (w - 1) + (before >= a - kTileStart ? 0 : 1)) * BQ;
+#pragma unroll
+  for (int i = 0; i < 16; i += kRows) {
+    const int r = x.row + blockIdx.y * 16 + i + tid / kLanes;
+    if (r >= x.n || tid / kLanes >= kRows) continue;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f, m = -INFINITY;
-    auto slot = [&](int k) -> int64_t {
-      return ((int64_t)2 * (wa + k) + (k > 0 || wa * per >= a - kTileStart ? 0 : 1)) * BQ + r - x.row;
-    };
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[slot(k)].x);
-    if (m == -INFINITY) m = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const int64_t s = slot(k);
+    int64_t s = part0 + r - x.row;
+    int next = w;
+    while (true) {
       const float2 ml = p.part_ml[s];
-      const float e = __builtin_amdgcn_exp2f(ml.x - m);
-      l += e * ml.y;
-      o += e * *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * lane);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * lane);
+      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+      const float e0 = __builtin_amdgcn_exp2f(m - ref), e1 = __builtin_amdgcn_exp2f(ml.x - ref);
+      l = e0 * l + e1 * ml.y;
+      o = e0 * o + e1 * y;
+      m = m_new;
+      if (next > p.workers || p.runs[next].place >= end) break;
+      s = (int64_t)2 * next * BQ + r - x.row;
+      ++next;
     }
-    const int token = r / g;
-    T* orow = (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
-    store_run(orow + 4 * lane, o * (l > 0.f ? 1.f / l : 0.f));
+    store_run(out_row(x, b.head, r), o * (l > 0.f ? 1.f / l : 0.f));
   }
 }
 
@@ -1120,7 +1165,6 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   const int64_t most = std::min<int64_t>(p.b.n_seqs, p.b.n_rows) + (int64_t)p.b.n_rows * g / S::BQ;
   const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC + kTileStart);
   TL_REQUIRE(line * p.b.Hkv < (1LL << 30), "batch too large: row blocks x kv heads x table positions");
-  TL_REQUIRE(p.b.Hkv <= 65535, "more than 65535 kv heads");
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
   p.workers = (int)std::max<int64_t>(8, (int64_t)S::kPerCu * cus / 8 * 8);
   p.most_tiles = (int)most;
@@ -1128,19 +1172,21 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   const size_t mbytes = aligned256((size_t)p.workers * 2 * S::BQ * sizeof(float2));
   const size_t tbytes = aligned256((size_t)most * sizeof(PagedTile));
   void* ws;
-  const int rc = workspace(ctx, obytes + mbytes + tbytes + ((size_t)p.b.n_seqs + 2) * sizeof(int), &ws);
+  const size_t rbytes = aligned256((size_t)(p.workers + 1) * sizeof(PagedRun));
+  const int rc = workspace(ctx, obytes + mbytes + tbytes + rbytes + ((size_t)p.b.n_seqs + 2) * sizeof(int), &ws);
   if (rc) return rc;
   p.part_o = (float*)ws;
   p.part_ml = (float2*)((char*)ws + obytes);
   p.tiles = (PagedTile*)((char*)ws + obytes + mbytes);
-  int* total = (int*)((char*)ws + obytes + mbytes + tbytes);
+  p.runs = (PagedRun*)((char*)ws + obytes + mbytes + tbytes);
+  int* total = (int*)((char*)ws + obytes + mbytes + tbytes + rbytes);
   paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
   if (p.cap > 0.f)
     paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   else
     paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   paged_tile_join_kernel<T, D, S::BQ>
-      <<<dim3((unsigned)most, (unsigned)p.b.Hkv, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
+      <<<dim3((unsigned)p.workers, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
   return TL_OK;
 }
 
