@@ -76,17 +76,41 @@ struct Rows {
   }
 };
 
-// dma_load16 from a uniform base and a per-lane byte offset.
-__device__ __forceinline__ void dma_load16_at(const void* base, uint32_t offset, uint32_t lds) {
+// N direct loads of a wave, 16 bytes a lane each: load i takes base + 1024 i + offset[i] (per lane) to LDS at
+// lds + 1024 i + 16 lane (the instruction's offset counts on both sides). M0 holds the LDS address; it must
+// have been written one wait state before it is used.
+template <int N>
+__device__ __forceinline__ void dma_load16_rows(const void* base, const uint32_t* offset, uint32_t lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "loads at a time");
   uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "global_load_lds_dwordx4 %2, %3\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds), "v"(offset), "s"(base)
-      : "memory");
+  if constexpr (N == 1)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds), "s"(base), "v"(offset[0])
+        : "memory");
+  else if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %2\n\t"
+        "global_load_lds_dwordx4 %4, %2 offset:1024\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds), "s"(base), "v"(offset[0]), "v"(offset[1])
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %3, %2\n\t"
+        "global_load_lds_dwordx4 %4, %2 offset:1024\n\t"
+        "global_load_lds_dwordx4 %5, %2 offset:2048\n\t"
+        "global_load_lds_dwordx4 %6, %2 offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds), "s"(base), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
+        : "memory");
 }
 // Waits until at most n direct loads of the wave are in flight (n is uniform, a multiple of STEP).
 template <int STEP, int MOST>
@@ -103,12 +127,17 @@ __device__ __forceinline__ void wait_loads(int n) {
 template <typename T, int D, bool KEYS>
 __device__ __forceinline__ void load_block16(const void* src, uint32_t lds, int lane) {
   using R = Rows<T, D>;
+  constexpr int kLoads = 16 / R::kPerLoad, N = kLoads < 4 ? kLoads : 4;
   const int rr = lane / R::kPieces, c = lane % R::kPieces;
 #pragma unroll
-  for (int i = 0; i < 16 / R::kPerLoad; ++i) {
-    const int row = i * R::kPerLoad + rr;
-    const int sw = KEYS ? R::key_swizzle(row) : R::value_swizzle(row);
-    dma_load16_at(src, (uint32_t)(row * R::kBytes + ((c ^ sw) << 4)), lds + i * 1024);
+  for (int i = 0; i < kLoads; i += N) {
+    uint32_t offset[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int row = (i + k) * R::kPerLoad + rr;
+      offset[k] = (uint32_t)(rr * R::kBytes + ((c ^ (KEYS ? R::key_swizzle(row) : R::value_swizzle(row))) << 4));
+    }
+    dma_load16_rows<N>((const unsigned char*)src + i * 1024, offset, lds + i * 1024);
   }
 }
 
@@ -877,29 +906,33 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   }
   if (at >= stop) return;
 
-  // the wave's blocks of 16 positions in every chunk (keys' blocks, then values'), their pages looked up a
-  // chunk ahead; one that no row of the block of rows sees is read from page 0 (masked, and zeroed)
-  constexpr int kMine = (2 * KT + NW - 1) / NW;
-  int id[kMine];
-  bool bad = false;
-  auto look_up = [&](const Item& x, int c) {
-    ConstInts pages = const_ints(p.b.table) + (int64_t)x.seq * p.b.ld_table;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int pos = c * KC + 16 * ((i * NW + wave) % KT);
-      id[i] = uniform(pages[min(pos >> p.b.page_shift, p.b.cols - 1)]);
-    }
+  // Pages: a lane holds one entry of the item's row of the table, 64 from entry `first` on, from which the
+  // wave picks. `pages` looks ahead for the item whose chunks are queued next.
+  struct Pages {
+    int first, entry;
   };
-  auto issue = [&](const Item& x, int c, int stage) {
+  auto look_up = [&](const Item& x, int c) {
+    Pages t;
+    t.first = (c * KC) >> p.b.page_shift;
+    t.entry = p.b.table[(int64_t)x.seq * p.b.ld_table + min(t.first + lane, p.b.cols - 1)];
+    asm volatile("" : "+v"(t.entry));  // waited for here, not at each use, where the direct loads would be too
+    return t;
+  };
+  // Queues chunk c of an item: the wave's blocks of 16 positions (keys' blocks, then values'). One that no
+  // row of the block of rows sees is read from page 0 (masked, and zeroed).
+  constexpr int kMine = (2 * KT + NW - 1) / NW;
+  bool bad = false;
+  auto issue = [&](const Item& x, int c, int stage, const Pages& t) {
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int blk = i * NW + wave;
       if (2 * KT % NW != 0 && blk >= 2 * KT) break;
       const int j = blk % KT, pos = c * KC + 16 * j;
-      const bool use = pos < x.hi_pos && pos + 16 > x.lo_pos, ok = (uint32_t)id[i] < (uint32_t)p.b.n_pages;
+      const int id = __builtin_amdgcn_readlane(t.entry, (pos >> p.b.page_shift) - t.first);
+      const bool use = pos < x.hi_pos && pos + 16 > x.lo_pos, ok = (uint32_t)id < (uint32_t)p.b.n_pages;
       bad |= use && !ok;
       const int slot = pos & ((1 << p.b.page_shift) - 1);
-      const int64_t from = ((((int64_t)(use && ok ? id[i] : 0) * p.b.Hkv + x.h) << p.b.page_shift) + slot) * R::kBytes;
+      const int64_t from = ((((int64_t)(use && ok ? id : 0) * p.b.Hkv + x.h) << p.b.page_shift) + slot) * R::kBytes;
       const int lds = (int)ring0 + stage * 2 * kHalf + (blk / KT) * kHalf + j * 16 * R::kBytes;
       if (blk < KT) load_block16<T, D, true>(uniform((const unsigned char*)p.k + from), uniform(lds), lane);
       else load_block16<T, D, false>(uniform((const unsigned char*)p.v + from), uniform(lds), lane);
@@ -910,14 +943,12 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   Item x = item(begin);
   int stage = 0;
   bool first_item = true;
-  look_up(x, x.c0);
-  issue(x, x.c0, 0);
+  Pages pages = look_up(x, x.c0);
+  issue(x, x.c0, 0, pages);
   while (true) {
     const bool more = at < stop;
     Item next = x;
     if (more) next = item(at);
-    if (x.count > 1) look_up(x, x.c0 + 1);
-    else if (more) look_up(next, next.c0);
     const int h = x.h, n = x.n;
     // the position of the block's row r
     auto position = [&](int r) { return PREFIX ? x.base : x.base + r / g; };
@@ -942,6 +973,8 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       m_run[i] = -INFINITY;
       l_part[i] = 0.f;
     }
+    Pages next_pages = pages;
+    if (more) next_pages = look_up(next, next.c0);
 #pragma unroll
     for (int k = 0; k < RG * M::KS; ++k)
       asm volatile("" : "+v"(qf[k].x), "+v"(qf[k].y), "+v"(qf[k].z), "+v"(qf[k].w));
@@ -957,10 +990,12 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       unsigned char* vals = ring[stage] + kHalf;
       stage ^= 1;
       dma_stage_sync<0>();  // this chunk has landed, and every wave is done with the other buffer
-      if (ch + 1 < x.count) issue(x, x.c0 + ch + 1, stage);
-      else if (more) issue(next, next.c0, stage);
-      if (ch + 2 < x.count) look_up(x, x.c0 + ch + 2);
-      else if (ch + 2 == x.count && more) look_up(next, next.c0);
+      if (ch + 1 < x.count) {
+        if (((k0 + 2 * KC - 1) >> p.b.page_shift) - pages.first >= 64) pages = look_up(x, x.c0 + ch + 1);
+        issue(x, x.c0 + ch + 1, stage, pages);
+      } else if (more) {
+        issue(next, next.c0, stage, next_pages);
+      }
       if (k0 < x.lo_pos || k0 + KC > x.hi_pos) {
         // positions that no row of the block sees may hold anything, and 0 times a NaN would be one
         for (int y = tid; y < KC * R::kPieces; y += 64 * NW) {
@@ -1032,6 +1067,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     first_item = false;
     if (!more) break;
     x = next;
+    pages = next_pages;
   }
   if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
