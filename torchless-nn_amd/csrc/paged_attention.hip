@@ -209,6 +209,32 @@ struct Tile16 {
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
     return __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
   }
+  // The bf16 operand P^T of a group's two tiles of 16 keys, s[0] and s[RG]
+  template <int RG>
+  __device__ __forceinline__ static bf16x8 weights(const f32x4* s) {
+    bf16x8 p;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = (__bf16)s[0][r];
+      p[4 + r] = (__bf16)s[RG][r];
+    }
+    return p;
+  }
+  // The same for OT output tiles from tile t0 on and operands p[2][RG] of 64 keys (bf16)
+  template <int RG, int OT>
+  __device__ __forceinline__ static void values_of(const unsigned char* vals, int t0, const bf16x8* p, f32x4* o, int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int t = 0; t < OT; ++t) {
+        const bf16x8 vf = value_frag(vals, c, t0 + t, lane);
+#pragma unroll
+        for (int i = 0; i < RG; ++i)
+          o[i * OT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[c * RG + i], o[i * OT + t], 0, 0, 0);
+      }
+    pipeline<2 * OT, 5, RG, 2>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
   // O^T += V^T P^T over KT tiles of 16 keys: s[tile][group], o[group][DT]
   template <int KT, int RG>
   __device__ __forceinline__ static void values(const unsigned char* vals, const f32x4* s, f32x4* o, int lane) {
@@ -217,12 +243,7 @@ struct Tile16 {
       for (int c = 0; c < KT / 2; ++c) {
         bf16x8 pf[RG];
 #pragma unroll
-        for (int i = 0; i < RG; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            pf[i][r] = (__bf16)s[2 * c * RG + i][r];
-            pf[i][4 + r] = (__bf16)s[(2 * c + 1) * RG + i][r];
-          }
+        for (int i = 0; i < RG; ++i) pf[i] = weights<RG>(s + 2 * c * RG + i);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const bf16x8 vf = value_frag(vals, c, t, lane);
@@ -825,14 +846,26 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
 // The same for a shared prefix (PREFIX): all rows of the batch as one sequence that sees positions 0 ..
 // skip - 1 whole, each workgroup one part of them for one block of rows; always parts, which the step
 // kernel's join takes in.
-template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PREFIX>
+//
+// PAIR (bf16 at D 256): two waves share RG x 16 rows. Each takes the scores of one half of a chunk's keys and
+// the outputs of one half of D, so that a key or value read from LDS serves two groups of rows without the
+// outputs of both over all of D in one wave's registers (which leave no room for a second wave on the SIMD).
+// They exchange their probabilities through LDS. LDS reads, 128 bytes a cycle, are what bounds the products:
+// with 16 rows a wave they took 4000 of a chunk's 7000 cycles.
+template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PREFIX, bool PAIR>
 __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const int* total) {
   using R = Rows<T, D>;
   using M = Tile16<T, D>;
-  constexpr int KT = KC / 16, BQ = 16 * RG * NW, kHalf = KC * R::kBytes;
+  constexpr int KT = KC / 16, BQ = 16 * RG * (PAIR ? NW / 2 : NW), kHalf = KC * R::kBytes;
+  constexpr int KTW = PAIR ? KT / 2 : KT, OT = PAIR ? M::DT / 2 : M::DT;  // a wave's key tiles and output tiles
+  static_assert(!PAIR || (KT == 4 && M::kBf), "pairs take 64 keys in bf16");
+  __shared__ uint4 swap_p[PAIR ? NW * RG * 64 : 1];
+  __shared__ float swap_m[PAIR ? NW : 1][RG][16];
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2][2 * kHalf];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int g = p.b.Hq / p.b.Hkv;
+  const int row_wave = PAIR ? wave % (NW / 2) : wave, half = PAIR ? wave / (NW / 2) : 0;  // a pair's are on one SIMD
+  const int other = PAIR ? wave ^ (NW / 2) : wave;
   // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
   const int w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
   const uint32_t ring0 = lds_offset(ring);
@@ -956,9 +989,9 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
     // this wave's rows
     uint4 qf[RG * M::KS];
     int pos_r[RG], lo_r[RG];
-    f32x4 o[RG * M::DT];
+    f32x4 o[RG * OT];
     float m_run[RG], l_part[RG];
-    const int wrow = x.row + wave * 16 * RG;
+    const int wrow = x.row + row_wave * 16 * RG;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
       const int r = min(wrow + 16 * i + fr, n - 1), token = r / g;
@@ -969,7 +1002,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       pos_r[i] = position(r);
       lo_r[i] = p.window > 0 ? max(0, pos_r[i] - p.window + 1) : 0;
 #pragma unroll
-      for (int t = 0; t < M::DT; ++t) o[i * M::DT + t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < OT; ++t) o[i * OT + t] = f32x4{0.f, 0.f, 0.f, 0.f};
       m_run[i] = -INFINITY;
       l_part[i] = 0.f;
     }
@@ -1004,15 +1037,20 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       }
-      if (!rows_here || k0 > pos_last || k0 + KC <= lo_first) continue;
-      f32x4 s[KT * RG];
-      M::template scores<KT, RG>(keys, qf, s, fr, fg);
-      const bool whole = k0 >= lo_last && k0 + KC <= pos_first + 1;
+      const bool sees = rows_here && k0 <= pos_last && k0 + KC > lo_first;
+      if (!sees) {
+        if constexpr (PAIR) asm volatile("s_barrier" ::: "memory");  // the one of the exchange below
+        continue;
+      }
+      const int kw = k0 + half * 16 * KTW;  // the wave's keys
+      f32x4 s[KTW * RG];
+      M::template scores<KTW, RG>(keys + half * 16 * KTW * R::kBytes, qf, s, fr, fg);
+      const bool whole = kw >= lo_last && kw + 16 * KTW <= pos_first + 1;
       float mx[RG];
       bool grow = false;
 #pragma unroll
       for (int i = 0; i < RG; ++i) {
-        mx[i] = mask_scores<T, CAP, KT, RG>(p, s + i, whole, k0 + 4 * fg, lo_r[i], pos_r[i]);
+        mx[i] = mask_scores<T, CAP, KTW, RG>(p, s + i, whole, kw + 4 * fg, lo_r[i], pos_r[i]);
         grow |= mx[i] > m_run[i] + 8.f;
       }
       if (__any(grow)) {
@@ -1020,13 +1058,14 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
         for (int i = 0; i < RG; ++i) {
           float v = fmaxf(mx[i], __shfl_xor(mx[i], 16, 64));
           v = fmaxf(v, __shfl_xor(v, 32, 64));
+          if constexpr (PAIR) v = ceilf(v);  // a whole power of two scales bf16 exactly, below
           const float m_new = v > m_run[i] + 8.f ? v : m_run[i];
           const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[i] - m_new);
           l_part[i] *= alpha;
 #pragma unroll
-          for (int t = 0; t < M::DT; ++t)
+          for (int t = 0; t < OT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[i * M::DT + t][r] *= alpha;
+            for (int r = 0; r < 4; ++r) o[i * OT + t][r] *= alpha;
           m_run[i] = m_new;
         }
       }
@@ -1034,7 +1073,7 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       for (int i = 0; i < RG; ++i) {
         const float m_ref = m_run[i] == -INFINITY ? 0.f : m_run[i];
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
+        for (int j = 0; j < KTW; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float y = __builtin_amdgcn_exp2f(s[j * RG + i][r] - m_ref);
@@ -1042,26 +1081,92 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
             l_part[i] += y;
           }
       }
-      M::template values<KT, RG>(vals, s, o, lane);
+      if constexpr (!PAIR) {
+        M::template values<KT, RG>(vals, s, o, lane);
+      } else {
+        bf16x8 pw[2 * RG];  // of both halves' keys
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+          const bf16x8 mine = M::template weights<RG>(s + i);
+          swap_p[(wave * RG + i) * 64 + lane] = __builtin_bit_cast(uint4, mine);
+          if (fg == 0) swap_m[wave][i][fr] = m_run[i];
+          pw[i] = pw[RG + i] = mine;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        float m_other[RG];
+        bool differ = false;
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+          const bf16x8 theirs = __builtin_bit_cast(bf16x8, swap_p[(other * RG + i) * 64 + lane]);
+          if (half) pw[i] = theirs;
+          else pw[RG + i] = theirs;
+          m_other[i] = swap_m[other][i][fr];
+          differ |= m_other[i] != m_run[i];
+        }
+        if (__any(differ)) {
+          // one of the two moved its maximum (rarely, once a row has seen a chunk): both go by the larger
+#pragma unroll
+          for (int i = 0; i < RG; ++i) {
+            const float m_new = fmaxf(m_run[i], m_other[i]), ref = m_new == -INFINITY ? 0.f : m_new;
+            const float mine = __builtin_amdgcn_exp2f(m_run[i] - ref), theirs = __builtin_amdgcn_exp2f(m_other[i] - ref);
+            const float first = half ? theirs : mine, second = half ? mine : theirs;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              pw[i][e] = (__bf16)((float)pw[i][e] * first);
+              pw[RG + i][e] = (__bf16)((float)pw[RG + i][e] * second);
+            }
+            l_part[i] *= mine;
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[i * OT + t][r] *= mine;
+            m_run[i] = m_new;
+          }
+        }
+        M::template values_of<RG, OT>(vals, half * OT, pw, o, lane);
+      }
     }
+    auto each_run = [&](int i, auto f) {
+      if constexpr (PAIR) {
+#pragma unroll
+        for (int t = 0; t < OT; ++t) f(16 * (half * OT + t) + 4 * fg, o[i * OT + t]);
+      } else {
+        M::each_run(o + i * OT, fg, f);
+      }
+    };
     const bool all = x.count == x.chunks;
     const int64_t slot = (PREFIX ? (int64_t)w : (int64_t)2 * w + (first_item ? 0 : 1)) * BQ;
     float* part_o = PREFIX ? p.pre_o : p.part_o;
     float2* part_ml = PREFIX ? p.pre_ml : p.part_ml;
+    if constexpr (PAIR) {
+      // the row's sum over both halves of the keys
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        l_part[i] += __shfl_xor(l_part[i], 16, 64);
+        l_part[i] += __shfl_xor(l_part[i], 32, 64);
+        swap_p[(wave * RG + i) * 64 + lane].x = __float_as_uint(l_part[i]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < RG; ++i) l_part[i] += __uint_as_float(swap_p[(other * RG + i) * 64 + lane].x);
+    }
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
-      float l = l_part[i] + __shfl_xor(l_part[i], 16, 64);
-      l += __shfl_xor(l, 32, 64);
+      float l = l_part[i];
+      if constexpr (!PAIR) {
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+      }
       const int r = wrow + 16 * i + fr, token = r / g;
       if (r >= n) continue;
       if (!PREFIX && all) {
         T* orow = (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(orow + d, y * inv); });
+        each_run(i, [&](int d, f32x4 y) { store_run(orow + d, y * inv); });
       } else {
         const int64_t at_row = slot + r - x.row;
-        M::each_run(o + i * M::DT, fg, [&](int d, f32x4 y) { store_run(part_o + at_row * D + d, y); });
-        if (fg == 0) part_ml[at_row] = make_float2(m_run[i], l);
+        each_run(i, [&](int d, f32x4 y) { store_run(part_o + at_row * D + d, y); });
+        if (fg == 0 && half == 0) part_ml[at_row] = make_float2(m_run[i], l);
       }
     }
     first_item = false;
@@ -1143,8 +1248,9 @@ struct StepShape {
 template <typename T, int D>
 struct TileShape {
   static constexpr bool kBf = sizeof(T) == 2;
-  static constexpr int NW = kBf && D == 256 ? 8 : 4, RG = kBf && D < 256 ? 2 : 1, KC = kBf ? 64 : 32;
-  static constexpr int BQ = 16 * NW * RG;
+  static constexpr int NW = kBf && D == 256 ? 8 : 4, RG = kBf ? 2 : 1, KC = kBf ? 64 : 32;
+  static constexpr bool kPair = kBf && D == 256;
+  static constexpr int BQ = 16 * RG * (kPair ? NW / 2 : NW);
   static constexpr int kLds = 4 * KC * D * (int)sizeof(T);
   static constexpr int kPerCu = std::min(160 * 1024 / kLds, kBf ? (D <= 32 ? 4 : D == 64 ? 3 : 2) : D <= 64 ? 4 : 2);
 };
@@ -1183,9 +1289,9 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   if (p.skip > 0) {
     const unsigned grid = (unsigned)((blocks + 7) / 8 * 8);
     if (p.cap > 0.f)
-      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, true, true><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, true, true, P::kPair><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
     else
-      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, false, true><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, false, true, P::kPair><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
   }
   if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
   else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
@@ -1218,9 +1324,9 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   int* total = (int*)((char*)ws + obytes + mbytes + tbytes + rbytes);
   paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
   if (p.cap > 0.f)
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   else
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, false><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   paged_tile_join_kernel<T, D, S::BQ>
       <<<dim3((unsigned)p.workers, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
   return TL_OK;
