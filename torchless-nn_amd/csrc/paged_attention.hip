@@ -1023,12 +1023,17 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       unsigned char* vals = ring[stage] + kHalf;
       stage ^= 1;
       dma_stage_sync<0>();  // this chunk has landed, and every wave is done with the other buffer
-      if (ch + 1 < x.count) {
-        if (((k0 + 2 * KC - 1) >> p.b.page_shift) - pages.first >= 64) pages = look_up(x, x.c0 + ch + 1);
-        issue(x, x.c0 + ch + 1, stage, pages);
-      } else if (more) {
-        issue(next, next.c0, stage, next_pages);
-      }
+      // the next chunk's loads. They leave a CU at 64 bytes a cycle, and who queues them waits for that: of a
+      // pair one queues its own before the scores, one after them
+      auto queue = [&]() {
+        if (ch + 1 < x.count) {
+          if (((k0 + 2 * KC - 1) >> p.b.page_shift) - pages.first >= 64) pages = look_up(x, x.c0 + ch + 1);
+          issue(x, x.c0 + ch + 1, stage, pages);
+        } else if (more) {
+          issue(next, next.c0, stage, next_pages);
+        }
+      };
+      if (half == 0) queue();
       if (k0 < x.lo_pos || k0 + KC > x.hi_pos) {
         // positions that no row of the block sees may hold anything, and 0 times a NaN would be one
         for (int y = tid; y < KC * R::kPieces; y += 64 * NW) {
@@ -1039,12 +1044,14 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
       }
       const bool sees = rows_here && k0 <= pos_last && k0 + KC > lo_first;
       if (!sees) {
+        if (half) queue();
         if constexpr (PAIR) asm volatile("s_barrier" ::: "memory");  // the one of the exchange below
         continue;
       }
       const int kw = k0 + half * 16 * KTW;  // the wave's keys
       f32x4 s[KTW * RG];
       M::template scores<KTW, RG>(keys + half * 16 * KTW * R::kBytes, qf, s, fr, fg);
+      if (half) queue();
       const bool whole = kw >= lo_last && kw + 16 * KTW <= pos_first + 1;
       float mx[RG];
       bool grow = false;
