@@ -350,6 +350,8 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
 // workgroup), whatever the sequences' lengths are; a wave streams its run through an LDS ring of its
 // own (ST chunks, direct loads, no barrier), across the sequences' borders. A (sequence, kv head)
 // inside one run is finished there; the parts of one that is cut are joined by the second kernel.
+// Where the tables hold a few chunks a sequence at most, a wave takes one (sequence, kv head) whole
+// (WHOLE), and there is no second launch.
 
 // What a sequence's rows see: positions lo .. hi - 1, row i those up to base + i.
 struct StepSeq {
@@ -401,61 +403,82 @@ struct StepCursor {
   }
 };
 
-template <typename T, int D, int KC, int ST, bool CAP>
-__global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
+template <typename T, int D, int KC, int ST, bool CAP, bool WHOLE>
+__device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsigned char* ring) {
   using R = Rows<T, D>;
   using M = Tile16<T, D>;
   constexpr int KT = KC / 16, kHalf = KC * R::kBytes, kStage = 2 * kHalf;
   constexpr int kLoads = kHalf / 1024;  // direct loads for a chunk's keys, and for its values
-  __shared__ __attribute__((aligned(1024))) unsigned char ring[ST * kStage];
-  const int lane = threadIdx.x, fr = lane & 15, fg = lane >> 4;
-  const int w = blockIdx.x, g = p.b.Hq / p.b.Hkv;
+  const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
+  const int g = p.b.Hq / p.b.Hkv;
 
-  // this wave's run [begin, end) of the line of chunks, and where it begins
-  int total = 0, mine = 0;
-  PagedSeq raw = {};
-  for (int s = lane; s < p.b.n_seqs; s += 64) {
-    raw = paged_seq(p.b, s, false);
-    mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
-    total += mine;
-  }
-  total = uniform(wave_sum_int(total) * p.b.Hkv);
-  const int per = (int)(((uint32_t)total + p.workers - 1) / (uint32_t)p.workers);
-  const int begin = uniform(w * per), end = min(total, begin + uniform(per));
-  if (begin >= end) return;
   StepCursor<KC> ld;
-  {
-    int before = 0, s0 = 0, incl;
-    while (true) {
-      if (p.b.n_seqs > 64) {
-        mine = 0;
-        if (s0 + lane < p.b.n_seqs) {
-          raw = paged_seq(p.b, s0 + lane, false);
-          mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
-        }
+  int begin, end;
+  if constexpr (WHOLE) {
+    ld.s = w / p.b.Hkv;
+    ld.h = w - ld.s * p.b.Hkv;
+    const PagedSeq raw = paged_seq(p.b, ld.s, ld.h == 0 && lane == 0);
+    ld.q = step_seq(p, uniform(raw.row0), uniform(raw.n), uniform(raw.len));
+    if (raw.n > p.max_q && lane == 0) latch(p.b.status, kBadSequence);
+    ld.c = ld.q.lo / KC;
+    begin = 0;
+    end = step_chunks<KC>(ld.q);
+    if (end == 0) {
+      // rows that see nothing
+      for (int x = lane; x < ld.q.n * g * (D / 4); x += 64) {
+        const int r = x / (D / 4), token = r / g;
+        store_run((T*)p.out + (int64_t)(ld.q.row0 + token) * p.ld_out + (ld.h * g + r - token * g) * D + 4 * (x % (D / 4)),
+                  f32x4{0.f, 0.f, 0.f, 0.f});
       }
-      incl = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += x;
-      }
-      const uint64_t past = __ballot((before + incl) * p.b.Hkv > begin);
-      if (past) {
-        const int at = __ffsll((unsigned long long)past) - 1;
-        ld.s = uniform(s0 + at);
-        before = uniform(before + __shfl(incl - mine, at, 64));
-        mine = uniform(__shfl(mine, at, 64));
-        ld.q = step_seq(p, uniform(__shfl(raw.row0, at, 64)), uniform(__shfl(raw.n, at, 64)), uniform(__shfl(raw.len, at, 64)));
-        break;
-      }
-      before += uniform(__shfl(incl, 63, 64));
-      s0 += 64;
-      if (s0 >= p.b.n_seqs) return;  // not reached: begin < total
+      return;
     }
-    const int off = begin - before * p.b.Hkv;
-    ld.h = uniform(off / mine);
-    ld.c = uniform(ld.q.lo / KC + off % mine);
+  } else {
+    // this wave's run [begin, end) of the line of chunks, and where it begins
+    int total = 0, mine = 0;
+    PagedSeq raw = {};
+    for (int s = lane; s < p.b.n_seqs; s += 64) {
+      raw = paged_seq(p.b, s, false);
+      mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
+      total += mine;
+    }
+    total = uniform(wave_sum_int(total) * p.b.Hkv);
+    const int per = (int)(((uint32_t)total + p.workers - 1) / (uint32_t)p.workers);
+    begin = uniform(w * per);
+    end = min(total, begin + uniform(per));
+    if (begin >= end) return;
+    {
+      int before = 0, s0 = 0, incl;
+      while (true) {
+        if (p.b.n_seqs > 64) {
+          mine = 0;
+          if (s0 + lane < p.b.n_seqs) {
+            raw = paged_seq(p.b, s0 + lane, false);
+            mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
+          }
+        }
+        incl = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int x = __shfl_up(incl, o, 64);
+          if (lane >= o) incl += x;
+        }
+        const uint64_t past = __ballot((before + incl) * p.b.Hkv > begin);
+        if (past) {
+          const int at = __ffsll((unsigned long long)past) - 1;
+          ld.s = uniform(s0 + at);
+          before = uniform(before + __shfl(incl - mine, at, 64));
+          mine = uniform(__shfl(mine, at, 64));
+          ld.q = step_seq(p, uniform(__shfl(raw.row0, at, 64)), uniform(__shfl(raw.n, at, 64)), uniform(__shfl(raw.len, at, 64)));
+          break;
+        }
+        before += uniform(__shfl(incl, 63, 64));
+        s0 += 64;
+        if (s0 >= p.b.n_seqs) return;  // not reached: begin < total
+      }
+      const int off = begin - before * p.b.Hkv;
+      ld.h = uniform(off / mine);
+      ld.c = uniform(ld.q.lo / KC + off % mine);
+    }
   }
   StepCursor<KC> cp = ld;
 
@@ -601,6 +624,12 @@ __global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
     cp.next(p);
   }
   if (bad && lane == 0) latch(p.b.status, kBadPage);
+}
+
+template <typename T, int D, int KC, int ST, bool CAP, bool WHOLE>
+__global__ __launch_bounds__(64) void paged_step_kernel(PagedAttn p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[ST * 2 * KC * Rows<T, D>::kBytes];
+  step_wave<T, D, KC, ST, CAP, WHOLE>(p, blockIdx.x, ring);
 }
 
 // Joins the parts of a row's query heads of one kv head: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,
@@ -852,22 +881,30 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
 // outputs of both over all of D in one wave's registers (which leave no room for a second wave on the SIMD).
 // They exchange their probabilities through LDS. LDS reads, 128 bytes a cycle, are what bounds the products:
 // with 16 rows a wave they took 4000 of a chunk's 7000 cycles.
+template <typename T, int D, int NW, int RG, int KC, bool PAIR>
+struct TileLds {
+  unsigned char ring[2][2 * KC * Rows<T, D>::kBytes];
+  uint4 swap_p[PAIR ? NW * RG * 64 : 1];
+  float swap_m[PAIR ? NW : 1][RG][16];
+};
+
 template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PREFIX, bool PAIR>
-__global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const int* total) {
+__device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total, const int block, const int blocks,
+                                           TileLds<T, D, NW, RG, KC, PAIR>& lds) {
   using R = Rows<T, D>;
   using M = Tile16<T, D>;
   constexpr int KT = KC / 16, BQ = 16 * RG * (PAIR ? NW / 2 : NW), kHalf = KC * R::kBytes;
   constexpr int KTW = PAIR ? KT / 2 : KT, OT = PAIR ? M::DT / 2 : M::DT;  // a wave's key tiles and output tiles
   static_assert(!PAIR || (KT == 4 && M::kBf), "pairs take 64 keys in bf16");
-  __shared__ uint4 swap_p[PAIR ? NW * RG * 64 : 1];
-  __shared__ float swap_m[PAIR ? NW : 1][RG][16];
-  __shared__ __attribute__((aligned(1024))) unsigned char ring[2][2 * kHalf];
+  auto& ring = lds.ring;
+  auto& swap_p = lds.swap_p;
+  auto& swap_m = lds.swap_m;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), fr = lane & 15, fg = lane >> 4;
   const int g = p.b.Hq / p.b.Hkv;
   const int row_wave = PAIR ? wave % (NW / 2) : wave, half = PAIR ? wave / (NW / 2) : 0;  // a pair's are on one SIMD
   const int other = PAIR ? wave ^ (NW / 2) : wave;
   // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
-  const int w = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
+  const int w = block % 8 * (blocks / 8) + block / 8;
   const uint32_t ring0 = lds_offset(ring);
 
   // the part of a block's chunks that the run holds: chunks c0 .. c0 + count - 1 of kv head h
@@ -1184,6 +1221,33 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
   if (bad && lane == 0) latch(p.b.status, kBadPage);
 }
 
+template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PAIR>
+__global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const int* total) {
+  __shared__ __attribute__((aligned(1024))) TileLds<T, D, NW, RG, KC, PAIR> lds;
+  tile_group<T, D, NW, RG, KC, CAP, false, PAIR>(p, total, blockIdx.x, gridDim.x, lds);
+}
+
+// A shared prefix and the sequences' own parts in one launch: the first is bound by the matrix cores, the
+// second by memory. Eight workgroups (one an XCD) of each kind take turns in the grid; one of the second
+// kind holds as many waves of the step kernel as its LDS has room for.
+template <typename T, int D, int NW, int RG, int KC, bool PAIR, int SKC, int SST, bool CAP>
+__global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int prefix_blocks, int step_blocks) {
+  using Lds = TileLds<T, D, NW, RG, KC, PAIR>;
+  constexpr int kRing = SST * 2 * SKC * Rows<T, D>::kBytes;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[sizeof(Lds) > kRing ? sizeof(Lds) : kRing];
+  constexpr int kWaves = sizeof(lds) / kRing < NW ? sizeof(lds) / kRing : NW;
+  const int round = blockIdx.x / 8, pre = prefix_blocks / 8, step = step_blocks / 8, both = min(pre, step);
+  const bool tile = round < 2 * both ? (round & 1) == 0 : pre > step;
+  const int block = (round < 2 * both ? round / 2 : round - both) * 8 + blockIdx.x % 8;
+  if (tile) {
+    tile_group<T, D, NW, RG, KC, CAP, true, PAIR>(p, nullptr, block, prefix_blocks, *reinterpret_cast<Lds*>(lds));
+  } else {
+    const int wave = uniform(threadIdx.x >> 6);
+    if (wave < kWaves && block * kWaves + wave < p.workers)
+      step_wave<T, D, SKC, SST, CAP, false>(p, block * kWaves + wave, lds + wave * kRing);
+  }
+}
+
 // Joins the parts of blocks that runs' borders cut, one workgroup per border and 16 rows (a block that
 // several cut is the first one's), and writes zeros for blocks that see nothing.
 template <typename T, int D, int BQ>
@@ -1248,6 +1312,11 @@ struct StepShape {
   static constexpr int ST = kRow * KC * 2 > 16384 ? 2 : 3;
   static constexpr int kLds = ST * 2 * KC * kRow;
   static constexpr int kPerCu = (160 * 1024) / kLds < 8 ? (160 * 1024) / kLds : 8;
+  // Chunks that one wave takes whole rather than share them out and join the parts, when there are few
+  // sequences and when there is one for each CU (us, whole / shared out: 65 keys x 4 heads fp32 at D 32 6.9 /
+  // 10.3; bf16, 2 heads at D 128: 16 x 128 to 256 keys 10.2 / 9.7, 128 x 64 to 256 11.1 / 14.5; 64 x 12 heads x 300
+  // to 512 at D 64 17.8 / 23.1; fp32's chunks take twice as long: 4 of 16 keys at D 256 13.7 / 11.7).
+  static constexpr int kWholeFew = sizeof(T) == 4 && D >= 128 ? 2 : 4, kWholeMany = 2 * kWholeFew;
 };
 
 // Blocks of the tile kernel: 128 rows, two 16-row groups a wave while their outputs fit the registers of
@@ -1271,17 +1340,32 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   const int64_t g = p.b.Hq / p.b.Hkv, rows = p.max_q * g, heads = (int64_t)p.b.n_rows * p.b.Hq;
   const int64_t most = (int64_t)p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
   TL_REQUIRE(most < (1LL << 30), "batch too large: sequences x kv heads x table positions");
+  const int64_t items = (int64_t)p.b.Hkv * p.b.n_seqs;
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
+  const int whole = items >= cus ? S::kWholeMany : S::kWholeFew;
+  if (p.shared == 0 && ((int64_t)p.b.cols << p.b.page_shift) <= whole * S::KC) {
+    p.skip = 0;
+    if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
+    else paged_step_kernel<T, D, S::KC, S::ST, false, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
+    return TL_OK;
+  }
   p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)S::kPerCu * cus));
   p.skip = p.shared;
-  int64_t blocks = 0;  // of the prefix kernel
   p.row_blocks = p.splits = 0;
+  int64_t blocks = 0, step_blocks = 0;
+  constexpr int kRing = S::kLds, kBlockLds = P::kLds > kRing ? P::kLds : kRing;
+  constexpr int kStepWaves = std::min(kBlockLds / kRing, P::NW);  // of a workgroup
   if (p.skip > 0) {
+    // The prefix's chunks are split for as many workgroups as are resident, two chunks each at least (us, 64
+    // rows x 8 heads x 2048 positions at D 256, with the join: one chunk each 24.6, two 21.3)
     p.row_blocks = (int)((p.b.n_rows * g + P::BQ - 1) / P::BQ);
     const int64_t lines = (int64_t)p.row_blocks * p.b.Hkv, chunks = (p.skip + P::KC - 1) / P::KC;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, (int64_t)P::kPerCu * cus / lines));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(chunks / 2, (int64_t)P::kPerCu * cus / lines));
     blocks = lines * p.splits;
     TL_REQUIRE(blocks < (1LL << 30), "batch too large: row blocks x kv heads x prefix");
+    const int64_t slots = std::max(1, 160 * 1024 / kBlockLds / 2) * (int64_t)cus;  // half of the chip
+    p.workers = (int)std::min<int64_t>(p.workers, slots * kStepWaves);
+    step_blocks = (p.workers + kStepWaves - 1) / kStepWaves;
   }
   const int64_t slots = 2LL * p.workers * rows + (p.skip > 0 ? heads : 0), pre = blocks * P::BQ;
   const size_t obytes = aligned256((size_t)slots * D * sizeof(float)), mbytes = aligned256((size_t)slots * sizeof(float2));
@@ -1294,14 +1378,16 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   p.pre_o = (float*)((char*)ws + obytes + mbytes);
   p.pre_ml = (float2*)((char*)ws + obytes + mbytes + pbytes);
   if (p.skip > 0) {
-    const unsigned grid = (unsigned)((blocks + 7) / 8 * 8);
+    const int n = (int)((blocks + 7) / 8 * 8), m = (int)((step_blocks + 7) / 8 * 8);
     if (p.cap > 0.f)
-      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, true, true, P::kPair><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, S::ST, true><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
     else
-      paged_tile_kernel<T, D, P::NW, P::RG, P::KC, false, true, P::kPair><<<grid, 64 * P::NW, 0, ctx->stream>>>(p, nullptr);
+      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, S::ST, false><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
+  } else if (p.cap > 0.f) {
+    paged_step_kernel<T, D, S::KC, S::ST, true, false><<<p.workers, 64, 0, ctx->stream>>>(p);
+  } else {
+    paged_step_kernel<T, D, S::KC, S::ST, false, false><<<p.workers, 64, 0, ctx->stream>>>(p);
   }
-  if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true><<<p.workers, 64, 0, ctx->stream>>>(p);
-  else paged_step_kernel<T, D, S::KC, S::ST, false><<<p.workers, 64, 0, ctx->stream>>>(p);
   const dim3 join((unsigned)((int64_t)p.b.n_rows * p.b.Hkv), (unsigned)((g + 256 / D - 1) / (256 / D)));
   paged_join_kernel<T, D, S::KC, P::BQ><<<join, 256, 0, ctx->stream>>>(p);
   return TL_OK;
@@ -1331,9 +1417,9 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   int* total = (int*)((char*)ws + obytes + mbytes + tbytes + rbytes);
   paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
   if (p.cap > 0.f)
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   else
-    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
+    paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   paged_tile_join_kernel<T, D, S::BQ>
       <<<dim3((unsigned)p.workers, S::BQ / 16), 256, 0, ctx->stream>>>(p, total);
   return TL_OK;
