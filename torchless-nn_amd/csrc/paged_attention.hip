@@ -1230,10 +1230,10 @@ __global__ __launch_bounds__(64 * NW) void paged_tile_kernel(PagedAttn p, const 
 // A shared prefix and the sequences' own parts in one launch: the first is bound by the matrix cores, the
 // second by memory. Eight workgroups (one an XCD) of each kind take turns in the grid; one of the second
 // kind holds as many waves of the step kernel as its LDS has room for.
-template <typename T, int D, int NW, int RG, int KC, bool PAIR, int SKC, int SST, bool CAP>
+template <typename T, int D, int NW, int RG, int KC, bool PAIR, int SKC, bool CAP>
 __global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int prefix_blocks, int step_blocks) {
   using Lds = TileLds<T, D, NW, RG, KC, PAIR>;
-  constexpr int kRing = SST * 2 * SKC * Rows<T, D>::kBytes;
+  constexpr int kRing = 2 * 2 * SKC * Rows<T, D>::kBytes;  // two chunks
   __shared__ __attribute__((aligned(1024))) unsigned char lds[sizeof(Lds) > kRing ? sizeof(Lds) : kRing];
   constexpr int kWaves = sizeof(lds) / kRing < NW ? sizeof(lds) / kRing : NW;
   const int round = blockIdx.x / 8, pre = prefix_blocks / 8, step = step_blocks / 8, both = min(pre, step);
@@ -1244,7 +1244,7 @@ __global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int 
   } else {
     const int wave = uniform(threadIdx.x >> 6);
     if (wave < kWaves && block * kWaves + wave < p.workers)
-      step_wave<T, D, SKC, SST, CAP, false>(p, block * kWaves + wave, lds + wave * kRing);
+      step_wave<T, D, SKC, 2, CAP, false>(p, block * kWaves + wave, lds + wave * kRing);
   }
 }
 
@@ -1353,7 +1353,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   p.skip = p.shared;
   p.row_blocks = p.splits = 0;
   int64_t blocks = 0, step_blocks = 0;
-  constexpr int kRing = S::kLds, kBlockLds = P::kLds > kRing ? P::kLds : kRing;
+  constexpr int kRing = 2 * 2 * S::KC * S::kRow, kBlockLds = P::kLds > kRing ? P::kLds : kRing;
   constexpr int kStepWaves = std::min(kBlockLds / kRing, P::NW);  // of a workgroup
   if (p.skip > 0) {
     // The prefix's chunks are split for as many workgroups as are resident, two chunks each at least (us, 64
@@ -1380,9 +1380,9 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   if (p.skip > 0) {
     const int n = (int)((blocks + 7) / 8 * 8), m = (int)((step_blocks + 7) / 8 * 8);
     if (p.cap > 0.f)
-      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, S::ST, true><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
+      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, true><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
     else
-      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, S::ST, false><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
+      paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, false><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
   } else if (p.cap > 0.f) {
     paged_step_kernel<T, D, S::KC, S::ST, true, false><<<p.workers, 64, 0, ctx->stream>>>(p);
   } else {
