@@ -25,6 +25,7 @@ struct PagedAttn {
   const void* v;
   void* out;
   int64_t ld_q, ld_out;
+  int g;              // query heads of a kv head
   int max_q, window;  // window 0: none
   int shared, skip;   // positions that the sequences share, and those of them that another kernel takes
   float scale;                // scores to log2 units: log2(e) / divisor, and with a cap
@@ -36,7 +37,7 @@ struct PagedAttn {
   // the shared prefix: its chunks cut into `splits` for each of row_blocks blocks of the batch's rows
   float* pre_o;
   float2* pre_ml;
-  int splits, row_blocks;
+  int splits, row_blocks;  // (without a prefix: most blocks of 16 rows that a sequence has)
   // the tile kernel's plan: row blocks of the batch, in order; per kv head they are one line of chunks
   PagedTile* tiles;
   PagedRun* runs;  // [workers + 1]
@@ -344,8 +345,8 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
 // ---------------------------------------------------------------------------------------
 // the step kernel
 // ---------------------------------------------------------------------------------------
-// Few rows a sequence (at most 16 of a kv head's query heads together): every key and value is read
-// once and used by one MFMA operand, so memory is the bound. The keys of all sequences and kv heads,
+// Few rows a sequence (kv head's query heads and tokens together), in blocks of 16: every key and value read
+// is used by one MFMA operand, so memory is the bound. The keys of all sequences and kv heads,
 // in chunks of KC, are one line that is cut into equal runs, one for each wave of the chip (a
 // workgroup), whatever the sequences' lengths are; a wave streams its run through an LDS ring of its
 // own (ST chunks, direct loads, no barrier), across the sequences' borders. A (sequence, kv head)
@@ -353,9 +354,9 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
 // Where the tables hold a few chunks a sequence at most, a wave takes one (sequence, kv head) whole
 // (WHOLE), and there is no second launch.
 
-// What a sequence's rows see: positions lo .. hi - 1, row i those up to base + i.
+// What a sequence's rows see: positions lo .. hi - 1, token i those up to base + i. `blocks`: of 16 rows.
 struct StepSeq {
-  int row0, n, base, lo, hi;
+  int row0, n, base, lo, hi, blocks;
 };
 __device__ __forceinline__ StepSeq step_seq(const PagedAttn& p, int row0, int n, int len) {
   StepSeq s;
@@ -364,6 +365,7 @@ __device__ __forceinline__ StepSeq step_seq(const PagedAttn& p, int row0, int n,
   s.base = len - n;
   s.lo = max(p.skip, p.window > 0 ? s.base - p.window + 1 : 0);
   s.hi = s.base + s.n;
+  s.blocks = (s.n * p.g + 15) >> 4;
   if (s.n <= 0 || s.hi <= s.lo) s.lo = s.hi = 0;
   return s;
 }
@@ -400,11 +402,15 @@ __device__ __forceinline__ StepSeq step_seq_at(const PagedAttn& p, int s) {
 
 template <int KC>
 struct StepCursor {
-  int s, h, c;  // sequence, kv head, chunk
+  int s, h, rb, c;  // sequence, kv head, block of rows, chunk
   StepSeq q;
   __device__ __forceinline__ void next(const PagedAttn& p) {
     if (++c < (q.hi + KC - 1) / KC) return;
-    if (++h == p.b.Hkv) {
+    if (++rb == q.blocks) {
+      rb = 0;
+      ++h;
+    }
+    if (h == p.b.Hkv) {
       h = 0;
       do {
         if (++s >= p.b.n_seqs) return;
@@ -422,24 +428,28 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
   constexpr int KT = KC / 16, kHalf = KC * R::kBytes, kStage = 2 * kHalf;
   constexpr int kLoads = kHalf / 1024;  // direct loads for a chunk's keys, and for its values
   const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
-  const int g = p.b.Hq / p.b.Hkv;
+  const int g = p.g;
 
   StepCursor<KC> ld;
   int begin, end;
   if constexpr (WHOLE) {
-    ld.s = w / p.b.Hkv;
-    ld.h = w - ld.s * p.b.Hkv;
-    const PagedSeq raw = paged_seq(p.b, ld.s, ld.h == 0 && lane == 0);
+    const int item = w / p.row_blocks;
+    ld.rb = w - item * p.row_blocks;
+    ld.s = item / p.b.Hkv;
+    ld.h = item - ld.s * p.b.Hkv;
+    const PagedSeq raw = paged_seq(p.b, ld.s, ld.h == 0 && ld.rb == 0 && lane == 0);
     ld.q = step_seq(p, uniform(raw.row0), uniform(raw.n), uniform(raw.len));
     if (raw.n > p.max_q && lane == 0) latch(p.b.status, kBadSequence);
+    if (ld.rb >= ld.q.blocks) return;
     ld.c = ld.q.lo / KC;
     begin = 0;
     end = step_chunks<KC>(ld.q);
     if (end == 0) {
       // rows that see nothing
-      for (int x = lane; x < ld.q.n * g * (D / 4); x += 64) {
-        const int r = x / (D / 4), token = r / g;
-        store_run((T*)p.out + (int64_t)(ld.q.row0 + token) * p.ld_out + (ld.h * g + r - token * g) * D + 4 * (x % (D / 4)),
+      const int h = ld.h, r0 = ld.rb * 16;
+      for (int x = lane; x < min(16, ld.q.n * g - r0) * (D / 4); x += 64) {
+        const int r = r0 + x / (D / 4), token = r / g;
+        store_run((T*)p.out + (int64_t)(ld.q.row0 + token) * p.ld_out + (h * g + r - token * g) * D + 4 * (x % (D / 4)),
                   f32x4{0.f, 0.f, 0.f, 0.f});
       }
       return;
@@ -450,9 +460,10 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
     PagedSeq raw = {};
     for (int s = lane; s < p.b.n_seqs; s += 64) {
       raw = paged_seq(p.b, s, false);
-      mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
+      const StepSeq q = step_seq(p, raw.row0, raw.n, raw.len);
+      most = max(most, step_chunks<KC>(q));
+      mine = step_chunks<KC>(q) * q.blocks;
       total += mine;
-      most = max(most, mine);
     }
     total = uniform(wave_sum_int(total) * p.b.Hkv);
     const int per = step_run(p, total, uniform(wave_max_int(most)));
@@ -466,7 +477,8 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
           mine = 0;
           if (s0 + lane < p.b.n_seqs) {
             raw = paged_seq(p.b, s0 + lane, false);
-            mine = step_chunks<KC>(step_seq(p, raw.row0, raw.n, raw.len));
+            const StepSeq q = step_seq(p, raw.row0, raw.n, raw.len);
+            mine = step_chunks<KC>(q) * q.blocks;
           }
         }
         incl = mine;
@@ -480,7 +492,6 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
           const int at = __ffsll((unsigned long long)past) - 1;
           ld.s = uniform(s0 + at);
           before = uniform(before + __shfl(incl - mine, at, 64));
-          mine = uniform(__shfl(mine, at, 64));
           ld.q = step_seq(p, uniform(__shfl(raw.row0, at, 64)), uniform(__shfl(raw.n, at, 64)), uniform(__shfl(raw.len, at, 64)));
           break;
         }
@@ -488,9 +499,11 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
         s0 += 64;
         if (s0 >= p.b.n_seqs) return;  // not reached: begin < total
       }
-      const int off = begin - before * p.b.Hkv;
-      ld.h = uniform(off / mine);
-      ld.c = uniform(ld.q.lo / KC + off % mine);
+      const int off = begin - before * p.b.Hkv, chunks = step_chunks<KC>(ld.q);
+      const int block = uniform(off / chunks);
+      ld.h = ld.q.blocks == 1 ? block : block / ld.q.blocks;
+      ld.rb = block - ld.h * ld.q.blocks;
+      ld.c = ld.q.lo / KC + off - block * chunks;
     }
   }
   StepCursor<KC> cp = ld;
@@ -542,13 +555,14 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
   f32x4 o[M::DT];
   float m_run = -INFINITY, l_part = 0.f;
   bool fresh = true, first_item = true;
-  int c_first = cp.c, stage = 0, token = 0, head = 0;
+  int c_first = cp.c, stage = 0, token = 0, head = 0, row = 0;
   for (int it = 0; it < count; ++it) {
     if (fresh) {
-      // rows of the item: token fr / g, query head fr % g of the kv head's; the columns past them repeat the first
-      const bool row_ok = fr < cp.q.n * g;
-      token = row_ok ? fr / g : 0;
-      head = cp.h * g + (row_ok ? fr - token * g : 0);
+      // the lane's row: token row / g, query head row % g of the kv head's; the columns past them repeat the first
+      row = cp.rb * 16 + fr;
+      const bool row_ok = row < cp.q.n * g;
+      token = row_ok ? row / g : 0;
+      head = cp.h * g + (row_ok ? row - token * g : 0);
       const T* qr = (const T*)p.q + (int64_t)(cp.q.row0 + token) * p.ld_q + head * D;
 #pragma unroll
       for (int ks = 0; ks < M::KS; ++ks) qf[ks] = *reinterpret_cast<const uint4*>(qr + (4 * ks + fg) * R::kVec);
@@ -616,7 +630,7 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
       float l = l_part + __shfl_xor(l_part, 16, 64);
       l += __shfl_xor(l, 32, 64);
       const bool all = last && c_first == cp.q.lo / KC;
-      if (fr < cp.q.n * g) {
+      if (row < cp.q.n * g) {
         if (all && p.skip == 0) {
           T* orow = (T*)p.out + (int64_t)(cp.q.row0 + token) * p.ld_out + head * D;
           const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -624,8 +638,9 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
         } else {
           // a run has at most two items that it does not hold whole: the one it begins in, and its last;
           // whole ones that the prefix is still to be joined to come after those of all runs
-          const int64_t slot = all ? (int64_t)2 * p.workers * (p.max_q * g) + (int64_t)(cp.q.row0 + token) * p.b.Hq + head
-                                   : (int64_t)(2 * w + (first_item ? 0 : 1)) * (p.max_q * g) + fr;
+          const int rows = min(p.max_q * g, 16);
+          const int64_t slot = all ? (int64_t)2 * p.workers * rows + (int64_t)(cp.q.row0 + token) * p.b.Hq + head
+                                   : (int64_t)(2 * w + (first_item ? 0 : 1)) * rows + fr;
           float* orow = p.part_o + slot * D;
           M::each_run(o, fg, [&](int d, f32x4 x) { store_run(orow + d, x); });
           if (fg == 0) p.part_ml[slot] = make_float2(m_run, l);
@@ -658,7 +673,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   __shared__ f32x4 acc[kGroups][kLanes];
   __shared__ float2 accml[kGroups];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x / p.b.Hkv, hk = blockIdx.x - t * p.b.Hkv, g = p.b.Hq / p.b.Hkv;
+  const int t = blockIdx.x / p.b.Hkv, hk = blockIdx.x - t * p.b.Hkv, g = p.g;
   const bool reports = blockIdx.x == 0 && blockIdx.y == 0;
   // the row's sequence, and the chunks of all and of those before it
   if (tid == 0) found = -1;
@@ -666,9 +681,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   int all = 0, most = 0, mine = 0;
   for (int s = tid; s < p.b.n_seqs; s += 256) {
     const PagedSeq x = paged_seq(p.b, s, reports);
-    mine = step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
+    const StepSeq q = step_seq(p, x.row0, x.n, x.len);
+    most = max(most, step_chunks<KC>(q));
+    mine = step_chunks<KC>(q) * q.blocks;
     all += mine;
-    most = max(most, mine);
     if (x.row0 <= t && t < x.row0 + x.n) atomicMax(&found, s);
   }
   __syncthreads();
@@ -680,7 +696,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   } else {
     for (int s = tid; s < sq; s += 256) {
       const PagedSeq x = paged_seq(p.b, s, false);
-      before += step_chunks<KC>(step_seq(p, x.row0, x.n, x.len));
+      const StepSeq q = step_seq(p, x.row0, x.n, x.len);
+      before += step_chunks<KC>(q) * q.blocks;
     }
   }
   all = wave_sum_int(all);
@@ -704,20 +721,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   before = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
   most = max(max(sums[0][2], sums[1][2]), max(sums[2][2], sums[3][2]));
   const int chunks = step_chunks<KC>(q);
+  const int grp = tid / kLanes, at = tid % kLanes;
+  const int h = blockIdx.y * kHeads + grp / kPhases, phase = grp % kPhases;
+  const int row = i * g + min(h, g - 1), prow = t * g + min(h, g - 1);  // of the sequence's, of the batch's
   int own = 0, wa = 0;  // parts of the row's own chunks
   bool at_start = false;
   if (chunks > 0) {
     const int per = step_run(p, all, most);
-    const int a = before * p.b.Hkv + hk * chunks;
+    const int a = before * p.b.Hkv + (hk * q.blocks + row / 16) * chunks;
     wa = a / per;
     own = (a + chunks - 1) / per - wa + 1;
     at_start = a == wa * per;
   }
-  if (own == 1 && p.skip == 0) return;  // finished by the step kernel
-  const int rows = p.max_q * g, parts = own + (p.skip > 0 ? p.splits : 0);
-  const int grp = tid / kLanes, at = tid % kLanes;
-  const int h = blockIdx.y * kHeads + grp / kPhases, phase = grp % kPhases;
-  const int row = i * g + h, prow = t * g + h;
+  const bool done = own == 1 && p.skip == 0;  // finished by the step kernel
+  if (done && q.blocks == 1) return;
+  const int rows = min(p.max_q * g, 16), parts = done ? 0 : own + (p.skip > 0 ? p.splits : 0);
   const int64_t whole = (int64_t)2 * p.workers * rows + (int64_t)t * p.b.Hq + hk * g + h;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
@@ -725,7 +743,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 #pragma unroll 4
     for (int k = phase; k < parts; k += kPhases) {
       const bool pre = k >= own;  // the prefix's
-      const int64_t mine_at = own == 1 ? whole : (int64_t)(2 * (wa + k) + (k > 0 || at_start ? 0 : 1)) * rows + row;
+      const int64_t mine_at = own == 1 ? whole : (int64_t)(2 * (wa + k) + (k > 0 || at_start ? 0 : 1)) * rows + row % 16;
       const int64_t pre_at = ((int64_t)(hk * p.splits + k - own) * p.row_blocks + prow / PBQ) * PBQ + prow % PBQ;
       const int64_t s = pre ? pre_at : mine_at;
       const float2 ml = (pre ? p.pre_ml : p.part_ml)[s];
@@ -740,7 +758,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   acc[grp][at] = o;
   if (at == 0) accml[grp] = make_float2(m, l);
   __syncthreads();
-  if (phase == 0 && h < g) {
+  if (phase == 0 && h < g && !done) {
     float top = m;
 #pragma unroll
     for (int k = 1; k < kPhases; ++k) top = fmaxf(top, accml[grp + k].x);
@@ -780,7 +798,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
   __shared__ int carry;
   __shared__ int keep[kKeep];
   __shared__ int keep_at[kKeepTiles];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.b.Hq / p.b.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = p.g;
   // inclusive sum over the workgroup plus what went before; all threads call it
   auto scan = [&](int x) {
 #pragma unroll
@@ -917,7 +935,7 @@ __device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total,
   auto& swap_p = lds.swap_p;
   auto& swap_m = lds.swap_m;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), fr = lane & 15, fg = lane >> 4;
-  const int g = p.b.Hq / p.b.Hkv;
+  const int g = p.g;
   const int row_wave = PAIR ? wave % (NW / 2) : wave, half = PAIR ? wave / (NW / 2) : 0;  // a pair's are on one SIMD
   const int other = PAIR ? wave ^ (NW / 2) : wave;
   // workgroups go round the 8 XCDs; neighbouring runs read the same keys, so each XCD takes a stretch of them
@@ -1270,7 +1288,7 @@ __global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int 
 template <typename T, int D, int BQ>
 __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const int* total) {
   constexpr int kLanes = D / 4, kRows = 256 / kLanes < 16 ? 256 / kLanes : 16;
-  const int tid = threadIdx.x, g = p.b.Hq / p.b.Hkv, lane = tid % kLanes;
+  const int tid = threadIdx.x, g = p.g, lane = tid % kLanes;
   const int line = total[0], tiles = total[1], w = blockIdx.x + 1;
   auto out_row = [&](const PagedTile& x, int h, int r) {
     const int token = r / g;
@@ -1354,14 +1372,16 @@ template <typename T, int D>
 static int launch_step(tl_ctx* ctx, PagedAttn p) {
   using S = StepShape<T, D>;
   using P = TileShape<T, D>;
-  const int64_t g = p.b.Hq / p.b.Hkv, rows = p.max_q * g, heads = (int64_t)p.b.n_rows * p.b.Hq;
-  const int64_t most = (int64_t)p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
+  const int64_t g = p.g, rows = std::min<int64_t>(p.max_q * g, 16), heads = (int64_t)p.b.n_rows * p.b.Hq;
+  const int64_t blocks16 = (p.max_q * g + 15) / 16;
+  const int64_t most = blocks16 * p.b.Hkv * p.b.n_seqs * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC);
   TL_REQUIRE(most < (1LL << 30), "batch too large: sequences x kv heads x table positions");
-  const int64_t items = (int64_t)p.b.Hkv * p.b.n_seqs;
+  const int64_t items = blocks16 * p.b.Hkv * p.b.n_seqs;
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
   const int whole = items >= cus ? S::kWholeMany : S::kWholeFew;
   if (p.shared == 0 && ((int64_t)p.b.cols << p.b.page_shift) <= whole * S::KC) {
     p.skip = 0;
+    p.row_blocks = (int)blocks16;
     if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
     else paged_step_kernel<T, D, S::KC, S::ST, false, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
     return TL_OK;
@@ -1413,7 +1433,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
 template <typename T, int D>
 static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   using S = TileShape<T, D>;
-  const int64_t g = p.b.Hq / p.b.Hkv;
+  const int64_t g = p.g;
   const int64_t most = std::min<int64_t>(p.b.n_seqs, p.b.n_rows) + (int64_t)p.b.n_rows * g / S::BQ;
   const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC + kTileStart);
   TL_REQUIRE(line * p.b.Hkv < (1LL << 30), "batch too large: row blocks x kv heads x table positions");
@@ -1442,10 +1462,20 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   return TL_OK;
 }
 
+// The step kernel reads a sequence's keys once for each 16 rows, the tile kernel once for 128, after a plan and
+// with a join that costs more. Up to kStepRows rows the first is taken while what it reads again is little (us,
+// step / tile: 24 rows, 2000 keys, D 256 16.6 / 70.7; 48 sequences x 32 rows, 500 to 2048 keys 32.6 / 41.8, 64
+// rows 52.0 / 48.5; 6 x 4 heads x 32 rows, 20000 to 60000 keys, D 128 174 / 139). Lengths are not known here:
+// what the tables hold stands for them.
+constexpr int kStepRows = 128;
+constexpr int64_t kStepAgain = 100 << 20;
+
 template <typename T, int D>
 static int launch_attention(tl_ctx* ctx, PagedAttn p) {
-  const int64_t g = p.b.Hq / p.b.Hkv;
-  if (p.max_q * g <= 16) return launch_step<T, D>(ctx, p);
+  const int64_t g = p.g;
+  const int64_t rows = p.max_q * g, again = (rows + 15) / 16 - 1;
+  const int64_t bytes = ((int64_t)p.b.n_seqs * p.b.cols << p.b.page_shift) * p.b.Hkv * D * 2 * (int64_t)sizeof(T);
+  if (rows <= 16 || (rows <= kStepRows && bytes <= kStepAgain / again)) return launch_step<T, D>(ctx, p);
   p.skip = 0;
   return launch_tiles<T, D>(ctx, p);
 }
@@ -1477,6 +1507,7 @@ extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const 
   if (rc) return rc;
   p.q = q; p.k = desc->k_pages; p.v = desc->v_pages; p.out = out;
   p.ld_q = ld_q; p.ld_out = ld_out;
+  p.g = p.b.Hq / p.b.Hkv;
   p.max_q = (int)std::min<int64_t>(max_q, desc->n_rows);
   p.window = (int)std::min<int64_t>(window, 1LL << 30);
   p.shared = (int)shared;
