@@ -1283,55 +1283,101 @@ __global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int 
   }
 }
 
-// Joins the parts of blocks that runs' borders cut, one workgroup per border and 16 rows (a block that
-// several cut is the first one's), and writes zeros for blocks that see nothing.
+// Joins the parts of blocks that runs' borders cut, and writes zeros for blocks that see nothing. A workgroup
+// belongs to a border and 16 rows of the block that it cuts; where a block is cut more than once the borders
+// share its rows, so that many parts have many workgroups.
 template <typename T, int D, int BQ>
 __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const int* total) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes < 16 ? 256 / kLanes : 16;
-  const int tid = threadIdx.x, g = p.g, lane = tid % kLanes;
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ f32x4 acc[kGroups][kLanes];
+  __shared__ float2 accml[kGroups];
+  const int tid = threadIdx.x, g = p.g, at = tid % kLanes, grp = tid / kLanes, lane = tid & 63;
   const int line = total[0], tiles = total[1], w = blockIdx.x + 1;
   auto out_row = [&](const PagedTile& x, int h, int r) {
     const int token = r / g;
-    return (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D + 4 * lane;
+    return (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D + 4 * at;
   };
   for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
     if (p.tiles[t].chunks > 0) continue;
     const PagedTile x = p.tiles[t];
     for (int h = 0; h < p.b.Hkv; ++h)
-      for (int i = tid / kLanes; i < 16; i += 256 / kLanes) {
+      for (int i = grp; i < 16; i += kGroups) {
         const int r = x.row + blockIdx.y * 16 + i;
         if (r < x.n) store_run(out_row(x, h, r), f32x4{0.f, 0.f, 0.f, 0.f});
       }
   }
   const PagedRun b = p.runs[w];
-  const int before = p.runs[w - 1].place;
   if (b.place >= line * p.b.Hkv) return;
   const PagedTile x = p.tiles[b.tile];
   const int a = b.head * line + x.at, end = a + x.chunks;
-  if (b.place <= a || b.place >= end || before > a) return;
+  if (b.place <= a || b.place >= end) return;
+  // borders of the same block before and after this one
+  int before = 0, after = 0;
+  while (true) {
+    const int i = w - 1 - before - lane;
+    const int n = __popcll(__ballot(i >= 0 && p.runs[max(i, 0)].place > a));
+    before += n;
+    if (n < 64) break;
+  }
+  while (true) {
+    const int i = w + 1 + after + lane;
+    const int n = __popcll(__ballot(i <= p.workers && p.runs[min(i, p.workers)].place < end));
+    after += n;
+    if (n < 64) break;
+  }
+  const int first = w - before, borders = before + 1 + after, parts = borders + 1;
   // the first part is its run's first item if no earlier block has chunks there; the others are
-  const int64_t part0 = (int64_t)(2 * (w - 1) + (before >= a - kTileStart ? 0 : 1)) * BQ;
+  const int64_t part0 = (int64_t)(2 * (first - 1) + (p.runs[first - 1].place >= a - kTileStart ? 0 : 1)) * BQ;
+  auto take = [&](int k, int r, f32x4& o, float& m, float& l) {
+    const int64_t s = (k == 0 ? part0 : (int64_t)2 * (first + k - 1) * BQ) + r - x.row;
+    const float2 ml = p.part_ml[s];
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * at);
+    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float e0 = __builtin_amdgcn_exp2f(m - ref), e1 = __builtin_amdgcn_exp2f(ml.x - ref);
+    l = e0 * l + e1 * ml.y;
+    o = e0 * o + e1 * y;
+    m = m_new;
+  };
+  if (parts <= 3) {
+    // a row a group, its parts one after another
 #pragma unroll
-  for (int i = 0; i < 16; i += kRows) {
-    const int r = x.row + blockIdx.y * 16 + i + tid / kLanes;
-    if (r >= x.n || tid / kLanes >= kRows) continue;
+    for (int i0 = 0; i0 < 16; i0 += kGroups) {
+      const int i = i0 + grp, r = x.row + blockIdx.y * 16 + i;
+      if (i >= 16 || r >= x.n || i % borders != before) continue;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float l = 0.f, m = -INFINITY;
+      take(0, r, o, m, l);
+      take(1, r, o, m, l);
+      if (parts == 3) take(2, r, o, m, l);
+      store_run(out_row(x, b.head, r), o * (l > 0.f ? 1.f / l : 0.f));
+    }
+    return;
+  }
+  for (int i = before; i < 16; i += borders) {
+    // a row, its parts round the groups
+    const int r = x.row + blockIdx.y * 16 + i;
+    if (r >= x.n) break;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f, m = -INFINITY;
-    int64_t s = part0 + r - x.row;
-    int next = w;
-    while (true) {
-      const float2 ml = p.part_ml[s];
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p.part_o + s * D + 4 * lane);
-      const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
-      const float e0 = __builtin_amdgcn_exp2f(m - ref), e1 = __builtin_amdgcn_exp2f(ml.x - ref);
-      l = e0 * l + e1 * ml.y;
-      o = e0 * o + e1 * y;
-      m = m_new;
-      if (next > p.workers || p.runs[next].place >= end) break;
-      s = (int64_t)2 * next * BQ + r - x.row;
-      ++next;
+#pragma unroll 4
+    for (int k = grp; k < parts; k += kGroups) take(k, r, o, m, l);
+    acc[grp][at] = o;
+    if (at == 0) accml[grp] = make_float2(m, l);
+    __syncthreads();
+    if (grp == 0) {
+      float top = m;
+      for (int k = 1; k < kGroups; ++k) top = fmaxf(top, accml[k].x);
+      const float ref = top == -INFINITY ? 0.f : top, e0 = __builtin_amdgcn_exp2f(m - ref);
+      l *= e0;
+      o *= e0;
+      for (int k = 1; k < kGroups; ++k) {
+        const float e = __builtin_amdgcn_exp2f(accml[k].x - ref);
+        l += e * accml[k].y;
+        o += e * acc[k][at];
+      }
+      store_run(out_row(x, b.head, r), o * (l > 0.f ? 1.f / l : 0.f));
     }
-    store_run(out_row(x, b.head, r), o * (l > 0.f ? 1.f / l : 0.f));
+    __syncthreads();
   }
 }
 
