@@ -1338,7 +1338,7 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const
     o = e0 * o + e1 * y;
     m = m_new;
   };
-  if (parts <= 3) {
+  if (parts <= (kGroups >= 8 ? kGroups / 2 : 3)) {
     // a row a group, its parts one after another
 #pragma unroll
     for (int i0 = 0; i0 < 16; i0 += kGroups) {
@@ -1348,7 +1348,8 @@ __global__ __launch_bounds__(256) void paged_tile_join_kernel(PagedAttn p, const
       float l = 0.f, m = -INFINITY;
       take(0, r, o, m, l);
       take(1, r, o, m, l);
-      if (parts == 3) take(2, r, o, m, l);
+#pragma unroll 2
+      for (int k = 2; k < parts; ++k) take(k, r, o, m, l);
       store_run(out_row(x, b.head, r), o * (l > 0.f ? 1.f / l : 0.f));
     }
     return;
