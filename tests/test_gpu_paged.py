@@ -411,3 +411,100 @@ def test_refusals(xp):
             xp.kv_append(**{**dict(qkv=qkv), **dev, **dict(n_heads_q=4), **kw})
     xp.synchronize()
     assert (out.get() == 0).all() and (big.get() == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 1, 256), (8, 2, 128), (12, 12, 64), (4, 4, 32)])
+def test_pieces_after_long_pasts(xp, dt, hq, hkv, d):
+    """Blocks of rows that see so many keys that many workgroups share them, beside short ones; rows in
+    blocks of 16 (a few a sequence) and in larger ones."""
+    for i, (lens, rows, kw) in enumerate([([6000, 300], [140, 5], {}), ([5000, 2100, 64], [9, 1, 16], dict(cap=20.0)),
+                                          ([4500], [200], dict(window=1000)), ([3100, 40], [33, 40], dict(cap=40.0))]):
+        rng = np.random.default_rng(d + i)
+        b = Batch(rng, lens, rows, hq, hkv, d, 64, dt, q_std=2.0)
+        _attend(xp, b, **kw)
+
+
+@pytest.mark.parametrize("d", [32, 256])
+def test_long_steps(xp, d):
+    """One sequence in more parts than are joined at a time, beside short ones and others without a row."""
+    rng = np.random.default_rng(17)
+    b = Batch(rng, [9000, 1, 500, 33, 70], [1, 1, 0, 1, 1], 8, 1, d, 128, "bf16", q_std=2.0)
+    _attend(xp, b)
+    _attend(xp, b, cap=10.0)
+    _attend(xp, b, window=3000)
+
+
+def test_very_many_sequences(xp):
+    """More sequences than a workgroup looks at in a round, with one long enough that its keys are shared
+    out; and more row blocks than the plan keeps at hand."""
+    rng = np.random.default_rng(18)
+    lens = [int(x) for x in rng.integers(1, 40, 700)]
+    lens[350] = 1500
+    b = Batch(rng, lens, [1] * 700, 4, 1, 32, 16, "bf16")
+    _attend(xp, b)
+    lens = [int(x) for x in rng.integers(0, 20, 4300)]
+    rows = [min(n, int(rng.integers(0, 3))) for n in lens]
+    lens[4000], rows[4000] = 300, 77
+    b = Batch(rng, lens, rows, 4, 2, 32, 16, "bf16", pad=3)
+    _attend(xp, b)
+
+
+@pytest.mark.parametrize("rows,shared", [(1, 0), (90, 0), (1, 64), (20, 0)])
+def test_outputs_in_the_queries_place(xp, rows, shared):
+    rng = np.random.default_rng(19)
+    b = Batch(rng, [400, 64 + rows, 200], [rows] * 3, 8, 2, 64, 16, "bf16", shared=shared)
+    dev = b.upload(xp)
+    pages = [dev[n] for n in ("k_pages", "v_pages", "page_table", "q_start", "kv_len")]
+    q = xp.array(b.q.reshape(b.n, -1), dtype="bf16")
+    want = xp.paged_attention(q, *pages, max_q=rows, divisor=8.0, shared=shared).get()
+    xp.paged_attention(q, *pages, max_q=rows, divisor=8.0, shared=shared, out=q)
+    assert np.array_equal(q.get(), want)
+
+
+def test_queries_as_columns_of_the_qkv_rows(xp):
+    """Without a rotation the queries are read where the product left them."""
+    rng = np.random.default_rng(20)
+    b = Batch(rng, [50, 20], [7, 20], 4, 2, 32, 16, "fp32")
+    x = rounded(rng.standard_normal((27, 8 * 32)), "fp32")
+    dev = b.upload(xp)
+    q = xp.kv_append(xp.array(x), **dev, n_heads_q=4)
+    assert q.pitch == 8 * 32
+    b.q = x[:, :128].reshape(27, 4, 32)
+    for s in range(2):
+        i = slice(b.start[s], b.start[s + 1])
+        r = b.rows[s]
+        b.keys[s][-r:], b.values[s][-r:] = x[i, 128:192].reshape(r, 2, 32), x[i, 192:].reshape(r, 2, 32)
+    out = xp.paged_attention(q, *(dev[n] for n in ("k_pages", "v_pages", "page_table", "q_start", "kv_len")), max_q=20,
+                             divisor=float(np.sqrt(32)))
+    want = b.want(float(np.sqrt(32)))
+    assert (np.abs(out.get().reshape(27, 4, 32) - want) <= b.tolerance(want)).all()
+
+
+def test_two_captured_batches_share_the_workspace(xp):
+    """Two graphs of different batches and an eager call between their replays use one workspace in turn."""
+    rng = np.random.default_rng(21)
+    made = []
+    for rows, lens in ((1, [900, 2000, 64]), (60, [700, 61, 1000])):
+        b = Batch(rng, lens, [rows] * 3, 8, 2, 128, 16, "bf16")
+        dev = b.upload(xp)
+        pages = [dev[n] for n in ("k_pages", "v_pages", "page_table", "q_start", "kv_len")]
+        q, out = xp.array(b.q.reshape(b.n, -1), dtype="bf16"), xp.empty((b.n, 8 * 128), "bf16")
+        call = lambda q=q, pages=pages, rows=rows, out=out: xp.paged_attention(  # noqa: E731
+            q, *pages, max_q=rows, divisor=11.0, out=out)
+        call()
+        made.append((call, out, out.get()))
+    graphs = []
+    for call, _, _ in made:
+        with xp.capture() as g:
+            call()
+        graphs.append(g)
+    for _ in range(3):
+        for g, (_, out, want) in zip(graphs, made):
+            out.fill(0)
+            g.launch()
+            made[0][0]()
+        for _, out, want in made:
+            assert np.array_equal(out.get(), want)
+    for g in graphs:
+        g.destroy()
