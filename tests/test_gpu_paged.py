@@ -508,3 +508,12 @@ def test_two_captured_batches_share_the_workspace(xp):
             assert np.array_equal(out.get(), want)
     for g in graphs:
         g.destroy()
+
+
+def test_a_border_moved_to_the_end_of_a_heads_blocks(xp):
+    """32 / 8 heads at D 128: on 256 CUs the blocks of 1300 rows (523 places a head) are cut into runs of 9, and
+    the 58th border, at 522, moves to the end of the first head's. The batch before leaves a block in the workspace
+    behind this one's last, which would lie across that place."""
+    rng = np.random.default_rng(22)
+    _attend(xp, Batch(rng, [640] * 41 + [3000], [1] * 41 + [60], 32, 8, 128, 64, "bf16", q_std=2.0))
+    _attend(xp, Batch(rng, [1300], [1300], 32, 8, 128, 64, "bf16", q_std=2.0))

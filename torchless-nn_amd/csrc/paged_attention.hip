@@ -899,6 +899,10 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttn p, int* tota
         }
       }
       r.place = r.head * line + off;
+      if (lo == tiles) {
+        lo = 0;  // the line's end is the next one's start
+        ++r.head;
+      }
       r.tile = lo;
     }
     p.runs[w] = r;
