@@ -924,7 +924,7 @@ template <typename T, int D, int NW, int RG, int KC, bool PAIR>
 struct TileLds {
   unsigned char ring[2][2 * KC * Rows<T, D>::kBytes];
   uint4 swap_p[PAIR ? NW * RG * 64 : 1];
-  float swap_m[PAIR ? NW : 1][RG][16];
+  float swap_m[PAIR ? NW : 1][RG][16], swap_l[PAIR ? NW : 1][RG][16];
 };
 
 template <typename T, int D, int NW, int RG, int KC, bool CAP, bool PREFIX, bool PAIR>
@@ -1222,16 +1222,17 @@ __device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total,
     float* part_o = PREFIX ? p.pre_o : p.part_o;
     float2* part_ml = PREFIX ? p.pre_ml : p.part_ml;
     if constexpr (PAIR) {
-      // the row's sum over both halves of the keys
+      // the row's sum over both halves of the keys (not by way of swap_p or swap_m, which the other wave may
+      // still be reading for the last chunk)
 #pragma unroll
       for (int i = 0; i < RG; ++i) {
         l_part[i] += __shfl_xor(l_part[i], 16, 64);
         l_part[i] += __shfl_xor(l_part[i], 32, 64);
-        swap_p[(wave * RG + i) * 64 + lane].x = __float_as_uint(l_part[i]);
+        if (fg == 0) lds.swap_l[wave][i][fr] = l_part[i];
       }
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < RG; ++i) l_part[i] += __uint_as_float(swap_p[(other * RG + i) * 64 + lane].x);
+      for (int i = 0; i < RG; ++i) l_part[i] += lds.swap_l[other][i][fr];
     }
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
