@@ -426,8 +426,8 @@ int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* qkv, int64_
 /* Causal attention of a ragged batch over its pages: out[t, h D ..] = sum_j p_j v_j over the
  * positions j <= p of row t's sequence (p the row's position), with window > 0 only those with
  * j > p - window; p = softmax of f(q . k_j / divisor), f(s) = softcap tanh(s / softcap) when
- * softcap > 0. q and out are [n_rows, Hq D] with row pitches ld_q and ld_out; query head h reads
- * kv head h / (Hq / Hkv). max_q is the most rows that a sequence of the batch has (more are
+ * softcap > 0 (bf16: up to 4096). q and out are [n_rows, Hq D] with row pitches ld_q and ld_out,
+ * and are the same rows or none in common; query head h reads kv head h / (Hq / Hkv). max_q is the most rows that a sequence of the batch has (more are
  * TL_ERR_BAD_INPUT, and the rest of that sequence is not written); it picks the kernel, so pass
  * 1 for a batch of single tokens. A row that sees no position gives zeros. Values at positions of
  * a sequence that its rows may not see reach no result, unless they are infinite or NaN and lie

@@ -38,15 +38,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, bool r
   return q;
 }
 
-// The page that holds position `pos` (within the table) of a sequence; page 0 for an index that the
-// cache does not have.
-__device__ __forceinline__ int paged_page(const PagedBatch& b, const int32_t* row, int pos, bool report) {
-  const int id = row[min(pos >> b.page_shift, b.cols - 1)];
-  if ((uint32_t)id < (uint32_t)b.n_pages) return id;
-  if (report) latch(b.status, kBadPage);
-  return 0;
-}
-
 // Reports, by a whole wave, a sequence that does not begin with the batch's `shared` first positions:
 // other pages than sequence 0's, or a row inside them.
 __device__ __forceinline__ void check_shared(const PagedBatch& b, int s, const PagedSeq& q, int shared, int lane) {
@@ -92,6 +83,5 @@ static void for_head_dim(int64_t d, F f) {
     default: f(HeadDim<256>{}); break;
   }
 }
-
 
 }  // namespace tl

@@ -304,8 +304,9 @@ __device__ __forceinline__ void store_run(bf16_t* p, f32x4 x) {
                                             (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16));
 }
 
-// A score in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), whose error of an fp32
-// rounding of c is far below bf16's steps; fp32 takes the library's tanh.
+// A score in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), off by a few fp32 roundings of
+// log2(e) c: up to c = 4096, the most that bf16 is served with, by some 2^-10, as a bf16 weight is by its own
+// rounding; fp32 takes the library's tanh.
 template <typename T, bool CAP>
 __device__ __forceinline__ float score(const PagedAttn& p, float s) {
   if constexpr (!CAP) return s * p.scale;
@@ -673,8 +674,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
   __shared__ f32x4 acc[kGroups][kLanes];
   __shared__ float2 accml[kGroups];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x / p.b.Hkv, hk = blockIdx.x - t * p.b.Hkv, g = p.g;
-  const bool reports = blockIdx.x == 0 && blockIdx.y == 0;
+  const int t = blockIdx.x, hk = blockIdx.z, g = p.g;
+  const bool reports = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
   // the row's sequence, and the chunks of all and of those before it
   if (tid == 0) found = -1;
   __syncthreads();
@@ -1431,7 +1432,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   const int64_t items = blocks16 * p.b.Hkv * p.b.n_seqs;
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
   const int whole = items >= cus ? S::kWholeMany : S::kWholeFew;
-  if (p.shared == 0 && ((int64_t)p.b.cols << p.b.page_shift) <= whole * S::KC) {
+  if (p.shared == 0 && items < (1LL << 26) && ((int64_t)p.b.cols << p.b.page_shift) <= whole * S::KC) {
     p.skip = 0;
     p.row_blocks = (int)blocks16;
     if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
@@ -1451,7 +1452,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
     const int64_t lines = (int64_t)p.row_blocks * p.b.Hkv, chunks = (p.skip + P::KC - 1) / P::KC;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(chunks / 2, (int64_t)P::kPerCu * cus / lines));
     blocks = lines * p.splits;
-    TL_REQUIRE(blocks < (1LL << 30), "batch too large: row blocks x kv heads x prefix");
+    TL_REQUIRE(blocks < (1LL << 22), "batch too large: row blocks x kv heads");
     const int64_t slots = std::max(1, 160 * 1024 / kBlockLds / 2) * (int64_t)cus;  // half of the chip
     p.workers = (int)std::min<int64_t>(p.workers, slots * kStepWaves);
     step_blocks = (p.workers + kStepWaves - 1) / kStepWaves;
@@ -1477,7 +1478,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   } else {
     paged_step_kernel<T, D, S::KC, S::ST, false, false><<<p.workers, 64, 0, ctx->stream>>>(p);
   }
-  const dim3 join((unsigned)((int64_t)p.b.n_rows * p.b.Hkv), (unsigned)((g + 256 / D - 1) / (256 / D)));
+  const dim3 join((unsigned)p.b.n_rows, (unsigned)((g + 256 / D - 1) / (256 / D)), (unsigned)p.b.Hkv);
   paged_join_kernel<T, D, S::KC, P::BQ><<<join, 256, 0, ctx->stream>>>(p);
   return TL_OK;
 }
@@ -1488,7 +1489,9 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   const int64_t g = p.g;
   const int64_t most = std::min<int64_t>(p.b.n_seqs, p.b.n_rows) + (int64_t)p.b.n_rows * g / S::BQ;
   const int64_t line = most * ((((int64_t)p.b.cols << p.b.page_shift) + S::KC - 1) / S::KC + kTileStart);
-  TL_REQUIRE(line * p.b.Hkv < (1LL << 30), "batch too large: row blocks x kv heads x table positions");
+  // (the second also when the bounds are wrong and sequences claim the same rows)
+  TL_REQUIRE(line * p.b.Hkv < (1LL << 30) && p.b.n_seqs * ((p.max_q * g + S::BQ - 1) / S::BQ) < (1LL << 31),
+             "batch too large: row blocks x kv heads x table positions");
   const int cus = ctx->num_cus > 0 ? ctx->num_cus : 256;
   p.workers = (int)std::max<int64_t>(8, (int64_t)S::kPerCu * cus / 8 * 8);
   p.most_tiles = (int)most;
@@ -1546,6 +1549,7 @@ extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const 
   if (rc) return rc;
   TL_REQUIRE(divisor > 0.f && divisor < INFINITY, "divisor must be positive and finite");
   TL_REQUIRE(softcap >= 0.f && softcap < INFINITY, "softcap must be 0 or positive and finite");
+  TL_REQUIRE(softcap <= 4096.f || desc->dtype != TL_BF16, "a softcap above 4096 is served in fp32 only");
   TL_REQUIRE(max_q > 0, "max_q must be positive");
   TL_REQUIRE(window >= 0, "negative window");
   TL_REQUIRE(shared >= 0 && shared % desc->page_size == 0 && shared <= desc->table_cols * desc->page_size,
@@ -1567,6 +1571,8 @@ extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const 
   p.scale = (float)(log2e / divisor);
   p.cap_in = softcap > 0.f ? (float)(2.0 * log2e / ((double)divisor * softcap)) : 0.f;
   p.cap = (float)(log2e * softcap);
+  TL_REQUIRE(p.scale > 0.f && p.scale < INFINITY && p.cap_in < INFINITY && p.cap < INFINITY &&
+             (softcap == 0.f || p.cap_in > 0.f), "divisor or softcap out of fp32's range");
   p.part_o = nullptr; p.part_ml = nullptr; p.workers = 0;
   const double es = (double)dtype_size(desc->dtype);
   // lengths are known on the device only: the profiler is told of the queries and outputs alone
