@@ -517,3 +517,19 @@ def test_a_border_moved_to_the_end_of_a_heads_blocks(xp):
     rng = np.random.default_rng(22)
     _attend(xp, Batch(rng, [640] * 41 + [3000], [1] * 41 + [60], 32, 8, 128, 64, "bf16", q_std=2.0))
     _attend(xp, Batch(rng, [1300], [1300], 32, 8, 128, 64, "bf16", q_std=2.0))
+
+
+def test_caps_and_divisors_out_of_range_are_refused(xp):
+    rng = np.random.default_rng(23)
+    for dt in ("bf16", "fp32"):
+        b = Batch(rng, [40, 9], [1, 1], 4, 2, 32, 16, dt, q_std=3.0)
+        dev = b.upload(xp)
+        q = xp.array(b.q.reshape(2, -1), dtype=dt)
+        pages = [dev[n] for n in ("k_pages", "v_pages", "page_table", "q_start", "kv_len")]
+        for kw in (dict(divisor=1e-39), dict(divisor=3.0, softcap=1e-39), dict(divisor=3.0, softcap=3e38),
+                   dict(divisor=3e38, softcap=4e3), *([dict(divisor=3.0, softcap=5000.0)] if dt == "bf16" else [])):
+            with pytest.raises(xp.TLError, match="softcap") as e:
+                xp.paged_attention(q, *pages, max_q=1, **kw)
+            assert e.value.status == xp.TL_ERR_INVALID
+        _attend(xp, b, cap=4096.0)
+        _attend(xp, b, cap=0.01)

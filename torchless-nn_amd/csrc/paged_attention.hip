@@ -1,6 +1,7 @@
 // Causal attention of a ragged batch over a paged KV cache (keys and values [page, kv head, slot, D],
 // both row-major): the step kernel for batches of few rows a sequence, and the join of its parts.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.hpp"
 
@@ -165,8 +166,14 @@ struct Tile16 {
   template <int KT, int RG>
   __device__ __forceinline__ static void scores(const unsigned char* keys, const uint4* q, f32x4* s, int fr, int fg) {
     const int sw = R::key_swizzle(fr);
+    // fp32: a sum of D products in chains of 64 at most, whose roundings are fewer than those of one chain and
+    // whose products wait for one another less
+    constexpr int C = kBf || D <= 64 ? 1 : D / 64;
+    f32x4 part[C][KT * RG];
 #pragma unroll
-    for (int i = 0; i < KT * RG; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < KT * RG; ++i) part[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -174,17 +181,24 @@ struct Tile16 {
         const uint4 k = *reinterpret_cast<const uint4*>(keys + (16 * j + fr) * R::kBytes + (((4 * ks + fg) ^ sw) << 4));
 #pragma unroll
         for (int i = 0; i < RG; ++i) {
-          f32x4& x = s[j * RG + i];
           if constexpr (kBf) {
+            f32x4& x = part[0][j * RG + i];
             x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
                                                         __builtin_bit_cast(bf16x8, q[i * KS + ks]), x, 0, 0, 0);
           } else {
             const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[i * KS + ks]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], x, 0, 0, 0);
+            for (int e = 0; e < 4; ++e)
+              part[e % C][j * RG + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], part[e % C][j * RG + i], 0, 0, 0);
           }
         }
       }
+#pragma unroll
+    for (int i = 0; i < KT * RG; ++i) {
+      s[i] = part[0][i];
+      if constexpr (C == 2) s[i] += part[1][i];
+      if constexpr (C == 4) s[i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
+    }
     pipeline<KT * KS, KT * KS < 6 ? KT * KS : 6, kBf ? RG : 4 * RG, 1>();
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -304,19 +318,26 @@ __device__ __forceinline__ void store_run(bf16_t* p, f32x4 x) {
                                             (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16));
 }
 
-// A score in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), off by a few fp32 roundings of
+// Scores as mask_scores leaves them: as they are, to be scaled to log2 units in the same fma that subtracts the
+// maximum (one rounding, at the size of the difference), or capped, in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), off by a few fp32 roundings of
 // log2(e) c: up to c = 4096, the most that bf16 is served with, by some 2^-10, as a bf16 weight is by its own
 // rounding; fp32 takes the library's tanh.
 template <typename T, bool CAP>
 __device__ __forceinline__ float score(const PagedAttn& p, float s) {
-  if constexpr (!CAP) return s * p.scale;
+  if constexpr (!CAP) return s;
   if constexpr (sizeof(T) == 4) return p.cap * tanhf(s * p.cap_in * 0.34657359027997264f);
   const float e = __builtin_amdgcn_exp2f(s * p.cap_in);
   return __builtin_fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(1.f + e), p.cap);
 }
 
-// The scores of KT x 16 keys from k0 on of one group (every RG-th of s) in log2 units, those of positions
-// outside lo .. hi at -inf unless all are inside (`whole`, uniform); returns the lane's largest.
+// 2^(score - m)
+template <bool CAP>
+__device__ __forceinline__ float weight(const PagedAttn& p, float s, float m) {
+  return __builtin_amdgcn_exp2f(CAP ? s - m : __builtin_fmaf(s, p.scale, -m));
+}
+
+// The scores of KT x 16 keys from k0 on of one group (every RG-th of s), those of positions outside lo .. hi
+// at -inf unless all are inside (`whole`, uniform); returns the lane's largest, in log2 units.
 template <typename T, bool CAP, int KT, int RG>
 __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool whole, int first, int lo, int hi) {
   float mx = -INFINITY;
@@ -340,7 +361,7 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
         mx = fmaxf(mx, s[j * RG][r]);
       }
   }
-  return mx;
+  return CAP ? mx : mx * p.scale;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -609,7 +630,7 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
     for (int j = 0; j < KT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - m_ref);
+        s[j][r] = weight<CAP>(p, s[j][r], m_ref);
         l_part += s[j][r];
       }
     wait_loads<kLoads, (2 * ST - 2) * kLoads>(ahead);
@@ -1160,7 +1181,7 @@ __device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total,
         for (int j = 0; j < KTW; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float y = __builtin_amdgcn_exp2f(s[j * RG + i][r] - m_ref);
+            const float y = weight<CAP>(p, s[j * RG + i][r], m_ref);
             s[j * RG + i][r] = y;
             l_part[i] += y;
           }
@@ -1571,8 +1592,8 @@ extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const 
   p.scale = (float)(log2e / divisor);
   p.cap_in = softcap > 0.f ? (float)(2.0 * log2e / ((double)divisor * softcap)) : 0.f;
   p.cap = (float)(log2e * softcap);
-  TL_REQUIRE(p.scale > 0.f && p.scale < INFINITY && p.cap_in < INFINITY && p.cap < INFINITY &&
-             (softcap == 0.f || p.cap_in > 0.f), "divisor or softcap out of fp32's range");
+  TL_REQUIRE(p.scale >= FLT_MIN && p.scale < INFINITY && p.cap_in < INFINITY && p.cap < INFINITY &&
+             (softcap == 0.f || p.cap_in >= FLT_MIN), "divisor or softcap out of fp32's range");
   p.part_o = nullptr; p.part_ml = nullptr; p.workers = 0;
   const double es = (double)dtype_size(desc->dtype);
   // lengths are known on the device only: the profiler is told of the queries and outputs alone
