@@ -2,6 +2,7 @@
 // both row-major): the step kernel for batches of few rows a sequence, and the join of its parts.
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 
 #include "paged.hpp"
 
@@ -29,8 +30,8 @@ struct PagedAttn {
   int g;              // query heads of a kv head
   int max_q, window;  // window 0: none
   int shared, skip;   // positions that the sequences share, and those of them that another kernel takes
-  float scale;                // scores to log2 units: log2(e) / divisor, and with a cap
-  float cap_in, cap;          // 2 log2(e) / (divisor softcap) and log2(e) softcap; cap 0: none
+  float scale;                // of score() to log2 units
+  float cap_in;               // of a product to score()'s argument; 0: no cap
   // the step kernel's parts, [slot][group rows]: outputs [D] and (max, sum)
   float* part_o;
   float2* part_ml;
@@ -318,22 +319,19 @@ __device__ __forceinline__ void store_run(bf16_t* p, f32x4 x) {
                                             (uint32_t)f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16));
 }
 
-// Scores as mask_scores leaves them: as they are, to be scaled to log2 units in the same fma that subtracts the
-// maximum (one rounding, at the size of the difference), or capped, in log2 units. Capped: c tanh(s / c) = c (1 - 2 / (1 + e^(2 s / c))), off by a few fp32 roundings of
-// log2(e) c: up to c = 4096, the most that bf16 is served with, by some 2^-10, as a bf16 weight is by its own
-// rounding; fp32 takes the library's tanh.
+// What `scale` turns into a score in log2 units, up to a constant of all a row's, in the same fma that takes
+// the maximum off (one rounding, at the size of the difference): a product of a query and a key, or where
+// scores are capped as c tanh(s / c), the tanh (fp32), or, as tanh x = 2 / (1 + e^(-2 x)) - 1, the fraction.
+// That is off by a few fp32 roundings of c: up to c = 4096, the most that bf16 is served with, by some 2^-10,
+// as a bf16 weight is by its own rounding.
 template <typename T, bool CAP>
 __device__ __forceinline__ float score(const PagedAttn& p, float s) {
   if constexpr (!CAP) return s;
-  if constexpr (sizeof(T) == 4) return p.cap * tanhf(s * p.cap_in * 0.34657359027997264f);
-  const float e = __builtin_amdgcn_exp2f(s * p.cap_in);
-  return __builtin_fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(1.f + e), p.cap);
+  if constexpr (sizeof(T) == 4) return tanhf(s * p.cap_in);
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * p.cap_in));
 }
-
-// 2^(score - m)
-template <bool CAP>
 __device__ __forceinline__ float weight(const PagedAttn& p, float s, float m) {
-  return __builtin_amdgcn_exp2f(CAP ? s - m : __builtin_fmaf(s, p.scale, -m));
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.scale, -m));
 }
 
 // The scores of KT x 16 keys from k0 on of one group (every RG-th of s), those of positions outside lo .. hi
@@ -361,7 +359,7 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
         mx = fmaxf(mx, s[j * RG][r]);
       }
   }
-  return CAP ? mx : mx * p.scale;
+  return mx * p.scale;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -630,7 +628,7 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
     for (int j = 0; j < KT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[j][r] = weight<CAP>(p, s[j][r], m_ref);
+        s[j][r] = weight(p, s[j][r], m_ref);
         l_part += s[j][r];
       }
     wait_loads<kLoads, (2 * ST - 2) * kLoads>(ahead);
@@ -1181,7 +1179,7 @@ __device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total,
         for (int j = 0; j < KTW; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float y = weight<CAP>(p, s[j * RG + i][r], m_ref);
+            const float y = weight(p, s[j * RG + i][r], m_ref);
             s[j * RG + i][r] = y;
             l_part[i] += y;
           }
@@ -1456,7 +1454,7 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   if (p.shared == 0 && items < (1LL << 26) && ((int64_t)p.b.cols << p.b.page_shift) <= whole * S::KC) {
     p.skip = 0;
     p.row_blocks = (int)blocks16;
-    if (p.cap > 0.f) paged_step_kernel<T, D, S::KC, S::ST, true, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
+    if (p.cap_in != 0.f) paged_step_kernel<T, D, S::KC, S::ST, true, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
     else paged_step_kernel<T, D, S::KC, S::ST, false, true><<<(unsigned)items, 64, 0, ctx->stream>>>(p);
     return TL_OK;
   }
@@ -1490,11 +1488,11 @@ static int launch_step(tl_ctx* ctx, PagedAttn p) {
   p.pre_ml = (float2*)((char*)ws + obytes + mbytes + pbytes);
   if (p.skip > 0) {
     const int n = (int)((blocks + 7) / 8 * 8), m = (int)((step_blocks + 7) / 8 * 8);
-    if (p.cap > 0.f)
+    if (p.cap_in != 0.f)
       paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, true><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
     else
       paged_shared_kernel<T, D, P::NW, P::RG, P::KC, P::kPair, S::KC, false><<<n + m, 64 * P::NW, 0, ctx->stream>>>(p, n, m);
-  } else if (p.cap > 0.f) {
+  } else if (p.cap_in != 0.f) {
     paged_step_kernel<T, D, S::KC, S::ST, true, false><<<p.workers, 64, 0, ctx->stream>>>(p);
   } else {
     paged_step_kernel<T, D, S::KC, S::ST, false, false><<<p.workers, 64, 0, ctx->stream>>>(p);
@@ -1529,7 +1527,7 @@ static int launch_tiles(tl_ctx* ctx, PagedAttn p) {
   p.runs = (PagedRun*)((char*)ws + obytes + mbytes + tbytes);
   int* total = (int*)((char*)ws + obytes + mbytes + tbytes + rbytes);
   paged_plan_kernel<S::BQ, S::KC><<<1, 1024, 0, ctx->stream>>>(p, total);
-  if (p.cap > 0.f)
+  if (p.cap_in != 0.f)
     paged_tile_kernel<T, D, S::NW, S::RG, S::KC, true, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
   else
     paged_tile_kernel<T, D, S::NW, S::RG, S::KC, false, S::kPair><<<p.workers, 64 * S::NW, 0, ctx->stream>>>(p, total);
@@ -1589,11 +1587,11 @@ extern "C" int tl_paged_attention(tl_ctx* ctx, const tl_paged_desc* desc, const 
   p.window = (int)std::min<int64_t>(window, 1LL << 30);
   p.shared = (int)shared;
   const double log2e = 1.4426950408889634;
-  p.scale = (float)(log2e / divisor);
-  p.cap_in = softcap > 0.f ? (float)(2.0 * log2e / ((double)divisor * softcap)) : 0.f;
-  p.cap = (float)(log2e * softcap);
-  TL_REQUIRE(p.scale >= FLT_MIN && p.scale < INFINITY && p.cap_in < INFINITY && p.cap < INFINITY &&
-             (softcap == 0.f || p.cap_in >= FLT_MIN), "divisor or softcap out of fp32's range");
+  const bool capped = softcap > 0.f, wide = desc->dtype == TL_F32;
+  p.scale = (float)(capped ? (wide ? 1.0 : 2.0) * log2e * softcap : log2e / divisor);
+  p.cap_in = capped ? (float)((wide ? 1.0 : -2.0 * log2e) / ((double)divisor * softcap)) : 0.f;
+  TL_REQUIRE(p.scale >= FLT_MIN && p.scale < INFINITY && std::fabs(p.cap_in) < INFINITY &&
+             (!capped || std::fabs(p.cap_in) >= FLT_MIN), "divisor or softcap out of fp32's range");
   p.part_o = nullptr; p.part_ml = nullptr; p.workers = 0;
   const double es = (double)dtype_size(desc->dtype);
   // lengths are known on the device only: the profiler is told of the queries and outputs alone
