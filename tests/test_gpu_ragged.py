@@ -162,3 +162,13 @@ def test_gpt_ragged(tl, dt):
             assert ref.max_rel(got[j], want) <= _tol(dt)
     with pytest.raises(ValueError):
         tl["gpt"].forward_ragged(net, np.array([[1]]), cache, cache.batch([ids[2]], [1]))
+
+
+def test_a_sequence_without_a_row_has_no_answer(tl):
+    model, _ = _gemma(tl, TINY, "bf16", 53)
+    cache = model.new_paged_cache(4, page_size=16)
+    seqs = [cache.add(), cache.add()]
+    for counts in ([1, 0], [2, 0]):
+        ids = tl["xp"].array(np.ones((1, sum(counts)), np.int64))
+        with pytest.raises(ValueError, match="no row"):
+            model.forward_ragged(ids, cache, cache.batch(seqs, counts))

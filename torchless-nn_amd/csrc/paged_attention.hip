@@ -1,5 +1,10 @@
-// Causal attention of a ragged batch over a paged KV cache (keys and values [page, kv head, slot, D],
-// both row-major): the step kernel for batches of few rows a sequence, and the join of its parts.
+// Causal attention of a ragged batch over a paged KV cache (keys and values [page, kv head, slot, D], both
+// row-major): the step kernel for few rows a sequence, the tile kernel for prompts, both in one launch for a
+// prefix that the sequences share, and the joins of their parts. For row t at position p of its sequence,
+//   out = sum_j 2^(s_j - m) v_j / l,  m = max_j s_j,  l = sum_j 2^(s_j - m),  p - window < j <= p,
+// in one pass over the keys: s in log2 units, m, l and the sums in fp32, moved along when m grows; parts of
+// the keys join by the same formula. bf16 rounds each weight 2^(s - m) once, as an operand of the matrix
+// cores, and the outputs.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

@@ -108,7 +108,7 @@ class GemmaDecoder:
         x = self.front.forward(ids)
         for i, blk in enumerate(self.blocks):
             x = blk.forward(x, cache, i, batch)
-        if batch.max_q > 1:
+        if not batch.single:
             last, C = batch.last_rows(), x.shape[-1]
             x = xp.embed(last, x.reshape(-1, C), None, last.size, out_shape=(1, last.size, C))
         return self.back.forward(self.final_norm.forward(x))

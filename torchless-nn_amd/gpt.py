@@ -108,7 +108,7 @@ def forward_ragged(net, ids, cache, batch):
         elif isinstance(layer, TransformerBlock):
             x = layer.forward(x, cache, i, batch)
             i += 1
-            if i == n_blocks and batch.max_q > 1:
+            if i == n_blocks and not batch.single:
                 last, C = batch.last_rows(), x.shape[-1]
                 x = xp.embed(last, x.reshape(-1, C), None, last.size, out_shape=(1, last.size, C))
         else:

@@ -529,6 +529,7 @@ class PagedBatch:
     def __init__(self, cache, seqs, counts, lengths, limits, shared):
         self.cache, self.seqs, self.counts, self.lengths = cache, tuple(seqs), tuple(counts), list(lengths)
         self.rows, self.max_q, self.shared = sum(counts), max([1, *counts]), shared
+        self.single = all(n == 1 for n in counts)  # a row a sequence: each its sequence's last
         self._limits = limits  # positions that each sequence's pages hold
         self._starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         table = np.zeros((len(seqs), max([1] + [len(cache.pages[s]) for s in seqs])), np.int32)
