@@ -427,11 +427,11 @@ int tl_kv_append(tl_ctx* ctx, const tl_paged_desc* desc, const void* qkv, int64_
  * positions j <= p of row t's sequence (p the row's position), with window > 0 only those with
  * j > p - window; p = softmax of f(q . k_j / divisor), f(s) = softcap tanh(s / softcap) when
  * softcap > 0 (bf16: up to 4096). q and out are [n_rows, Hq D] with row pitches ld_q and ld_out,
- * and are the same rows or none in common; query head h reads kv head h / (Hq / Hkv). max_q is the most rows that a sequence of the batch has (more are
- * TL_ERR_BAD_INPUT, and the rest of that sequence is not written); it picks the kernel, so pass
- * 1 for a batch of single tokens. A row that sees no position gives zeros. Values at positions of
- * a sequence that its rows may not see reach no result, unless they are infinite or NaN and lie
- * before a row of the same call that may.
+ * the same rows or none in common; query head h reads kv head h / (Hq / Hkv). max_q is the most
+ * rows that a sequence of the batch has (more are TL_ERR_BAD_INPUT, and the rest of that sequence
+ * is not written); it picks the kernel, so pass 1 for a batch of single tokens. A row that sees no
+ * position gives zeros. Keys and values at positions that a row may not see do not reach its
+ * result, whatever they hold.
  * shared > 0 (a multiple of page_size, no window): the sequences begin with the same `shared`
  * positions, held by the same pages (checked on the device), and every row lies behind them;
  * a batch of few rows then reads them once for all. Results are those of shared = 0 up to

@@ -533,3 +533,37 @@ def test_caps_and_divisors_out_of_range_are_refused(xp):
             assert e.value.status == xp.TL_ERR_INVALID
         _attend(xp, b, cap=4096.0)
         _attend(xp, b, cap=0.01)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 1, 256), (8, 2, 128), (12, 12, 64), (4, 4, 32)])
+def test_values_that_some_rows_may_not_see(xp, dt, hq, hkv, d):
+    """Infinite and NaN values (and keys) of the batch's own positions reach the rows that see them, and the
+    others' results are those of finite ones: later positions, and with a window those before it."""
+    rng = np.random.default_rng(d)
+    for lens, rows, window, cap in (([300, 90], [300, 40], 0, 0.0), ([700, 2000], [150, 180], 64, 0.0),
+                                    ([500, 60], [2, 9], 0, 20.0), ([500, 60], [2, 9], 33, 0.0), ([4000], [30], 0, 0.0)):
+        b = Batch(rng, lens, rows, hq, hkv, d, 16, dt, q_std=2.0)
+        hidden = np.zeros((b.n, b.hq), bool)
+        for s, (n, r) in enumerate(zip(lens, rows)):
+            pos = np.arange(n - r, n)
+            for j, what, which in ((n - 1, np.inf, "v"), (n - r // 3 - 1, np.nan, "kv"), (n - r, -np.inf, "v")):
+                if j == n - r and not window:
+                    continue  # all rows would see it
+                kv_at = [a[b.slots(s, [j])] for a in (b.k, b.v)]
+                bad = np.full_like(kv_at[1], what)
+                bad[..., 1::2] = kv_at[1][..., 1::2] if which == "v" else what
+                b.v[b.slots(s, [j])] = bad
+                if which == "kv":
+                    b.k[b.slots(s, [j])] = what
+                sees = (pos >= j) & ((pos < j + window) if window else True)
+                hidden[b.start[s]:b.start[s] + r] |= sees[:, None]
+        dev = b.upload(xp)
+        q, out = xp.array(b.q.reshape(b.n, -1), dtype=dt), xp.empty((b.n, hq * d), dt)
+        xp.paged_attention(q, dev["k_pages"], dev["v_pages"], dev["page_table"], dev["q_start"], dev["kv_len"],
+                           max_q=max(rows), divisor=float(np.sqrt(d)), softcap=cap, window=window, out=out)
+        got, want = out.get().reshape(b.n, hq, d), b.want(float(np.sqrt(d)), cap, window)
+        ok = ~hidden
+        assert ok.any() or window >= max(rows)  # (a window of all rows shows the first one's position to all)
+        assert (np.abs(got - want)[ok] <= b.tolerance(want)[ok]).all()
+        assert not np.isfinite(got[hidden]).all(-1).any()

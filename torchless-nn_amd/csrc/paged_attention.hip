@@ -298,6 +298,10 @@ struct Tile16 {
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+  // The output that element r of the lane's tile t is
+  __device__ __forceinline__ static int column(int t, int r, int fg) {
+    return kBf ? 16 * t + 4 * fg + r : 16 * E * (t / E) + 4 * E * fg + E * r + t % E;
+  }
   // Calls f(d, x) for runs of 4 consecutive outputs x of the lane's query row, at d .. d + 3 (fp32 at
   // D = 32: 2 runs of 4 all the same).
   template <typename F>
@@ -365,6 +369,56 @@ __device__ __forceinline__ float mask_scores(const PagedAttn& p, f32x4* s, bool 
       }
   }
   return mx * p.scale;
+}
+
+// Outputs that are NaN although the row's sum l is not: a position that another row of the wave sees, and this
+// one may not, holds an infinite or NaN value, and its weight 0 times that is NaN. (Or one that it may see does,
+// and then they stay what they are.) The lane's OT tiles from tile t0 on are summed again, key by key from memory
+// over positions from .. to - 1, without those outside lo .. pos. Slow, and not on any path of finite values.
+template <typename T, int D, bool CAP, int OT>
+__device__ __forceinline__ void mend(const PagedAttn& p, ConstInts table, int h, const uint4* q, f32x4* o, float l,
+                                     float m_run, int from, int to, int lo, int pos, int t0, int fg) {
+  using M = Tile16<T, D>;
+  using R = Rows<T, D>;
+  bool mine = false;
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mine |= o[t][r] != o[t][r];
+  mine = mine && l == l;
+  if (!__any(mine)) return;
+  const float m = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[t][r] = mine ? 0.f : o[t][r];
+#pragma unroll 1
+  for (int j = from; j < to; ++j) {
+    const int id = uniform(table[min(j >> p.b.page_shift, p.b.cols - 1)]);
+    const int slot = j & ((1 << p.b.page_shift) - 1);
+    const int64_t at = ((((int64_t)((uint32_t)id < (uint32_t)p.b.n_pages ? id : 0) * p.b.Hkv + h) << p.b.page_shift) + slot) * D;
+    float s = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < M::KS; ++ks) {
+      float a[R::kVec], b[R::kVec];
+      Elem<T>::unpack(q[ks], a);
+      Elem<T>::unpack(*reinterpret_cast<const uint4*>((const T*)p.k + at + (4 * ks + fg) * R::kVec), b);
+#pragma unroll
+      for (int e = 0; e < R::kVec; ++e) s = __builtin_fmaf(a[e], b[e], s);
+    }
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    const bool see = mine && j >= lo && j <= pos;
+    const float w = weight(p, score<T, CAP>(p, s), m);
+    const T* v = (const T*)p.v + at;
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = Elem<T>::load(v + M::column(t0 + t, r, fg));
+        o[t][r] = see ? __builtin_fmaf(w, x, o[t][r]) : o[t][r];
+      }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -655,6 +709,9 @@ __device__ __forceinline__ void step_wave(const PagedAttn& p, const int w, unsig
       float l = l_part + __shfl_xor(l_part, 16, 64);
       l += __shfl_xor(l, 32, 64);
       const bool all = last && c_first == cp.q.lo / KC;
+      if (cp.q.n > 1)  // (the rows of one token see the same)
+        mend<T, D, CAP, M::DT>(p, const_ints(p.b.table) + (int64_t)cp.s * p.b.ld_table, cp.h, qf, o, l, m_run,
+                               max(c_first * KC, cp.q.lo), min(k0 + KC, cp.q.hi), lo, pos, 0, fg);
       if (row < cp.q.n * g) {
         if (all && p.skip == 0) {
           T* orow = (T*)p.out + (int64_t)(cp.q.row0 + token) * p.ld_out + head * D;
@@ -1267,6 +1324,10 @@ __device__ __forceinline__ void tile_group(const PagedAttn& p, const int* total,
         l += __shfl_xor(l, 32, 64);
       }
       const int r = wrow + 16 * i + fr, token = r / g;
+      if constexpr (!PREFIX)
+        mend<T, D, CAP, OT>(p, const_ints(p.b.table) + (int64_t)x.seq * p.b.ld_table, h, qf + i * M::KS, o + i * OT, l,
+                            m_run[i], max(x.c0 * KC, x.lo_pos), min((x.c0 + x.count) * KC, x.hi_pos), lo_r[i], pos_r[i],
+                            half * OT, fg);
       if (r >= n) continue;
       if (!PREFIX && all) {
         T* orow = (T*)p.out + (int64_t)(x.row0 + token) * p.ld_out + (h * g + r - token * g) * D;
