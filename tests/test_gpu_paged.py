@@ -567,3 +567,13 @@ def test_values_that_some_rows_may_not_see(xp, dt, hq, hkv, d):
         assert ok.any() or window >= max(rows)  # (a window of all rows shows the first one's position to all)
         assert (np.abs(got - want)[ok] <= b.tolerance(want)[ok]).all()
         assert not np.isfinite(got[hidden]).all(-1).any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("hq,hkv,d", [(71, 1, 64), (17, 1, 256), (15, 5, 32), (10, 2, 128), (3, 3, 256), (66, 2, 32)])
+def test_odd_groups_of_heads(xp, dt, hq, hkv, d):
+    """Query heads a kv head that are no power of two, or more than a block of 16 rows holds."""
+    for i, (lens, rows, kw) in enumerate([([70, 1, 300], [1, 1, 1], {}), ([64 + 40, 64 + 3], [2, 1], dict(shared=64)),
+                                          ([90, 33], [50, 7], dict(cap=30.0)), ([200, 17], [5, 17], dict(window=40))]):
+        b = Batch(np.random.default_rng(i), lens, rows, hq, hkv, d, 32, dt, q_std=2.0, shared=kw.get("shared", 0))
+        _attend(xp, b, **kw)
