@@ -1142,8 +1142,8 @@ def paged_attention(q: DeviceTensor, k_pages: DeviceTensor, v_pages: DeviceTenso
                     shared=0, out=None) -> DeviceTensor:
     """Causal attention of a ragged batch's queries q [N, Hq D] over the pages of their sequences (the
     batch as in kv_append, its keys and values appended) -> [N, Hq D]. `max_q`: the most rows that a
-    sequence has here; `softcap` c > 0 caps scores as c tanh(s / c); `window` w > 0 lets position p see
-    p - w + 1 .. p only; `shared`: the sequences begin with this many positions (whole pages) in the
+    sequence has here; `softcap` c > 0 caps scores as c tanh(s / c) (bf16: c up to 4096);
+    `window` w > 0 lets position p see p - w + 1 .. p only; `shared`: the sequences begin with this many positions (whole pages) in the
     same pages, read once for all by a batch of few rows a sequence."""
     d = k_pages.shape[-1]
     n, wq = q.nrows, q.ncols
